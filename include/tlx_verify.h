@@ -458,6 +458,104 @@ int tlx_prefill_w4a8_gate_up(const void* w_gate, const void* w_up, const int8_t*
                              const float* sx, int m, int64_t n_rows, int64_t k, float* act, int64_t ld_act, void* ws,
                              size_t ws_bytes, void* stream);
 
+/* ---- paged serving: a KV cache shared by many requests ------------------------------
+ * No reference counterpart (the reference serves one request from one contiguous
+ * cache).  The cache is a pool of pages of page_size tokens (a power of two, 8..1024):
+ * k / v [page][kv_head][slot][head_dim], addressed by three strides each (elements), so
+ * that a [page][slot][kv_head][head_dim] pool is the same struct with other strides.
+ * dtype TLX_DT_F16, TLX_DT_BF16, or TLX_DT_Q8: uint8 codes (q + 128) with one fp16 scale
+ * per 32 dims, k_scale / v_scale [page][kv_head][slot][head_dim / 32], the element
+ * format of the contiguous int8 cache above; a code stands for fp16((code - 128) * scale).
+ * head_dim is 64, 128 or 256; base addresses and strides of k / v are multiples of 16
+ * bytes, those of the scales of head_dim / 16 bytes. */
+#define TLX_DT_Q8 102
+typedef struct tlx_paged_kv {
+  void* k;
+  void* v;
+  void* k_scale;           /* TLX_DT_Q8 only */
+  void* v_scale;
+  int64_t k_stride[3];     /* page, head, slot */
+  int64_t v_stride[3];
+  int64_t ks_stride[3];
+  int64_t vs_stride[3];
+  int64_t pages;           /* pages * page_size < 2^31 */
+  int32_t page_size;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t dtype;
+} tlx_paged_kv;
+
+/* Page planning on the device.  Request b has cached_len[b] tokens in the cache, brings
+ * new_len[b] more and holds held_in[b] pages, the first entries of block_table[b] (row
+ * stride table_stride >= table_width).  It needs ceil((cached + new) / page_size) pages;
+ * the missing ones come off the free stack free_pages[0 .. n_free) from the top, in
+ * request order, and are written behind the held ones (pages held beyond the need, after
+ * rejected drafts say, stay).  The first request that the free pages do not cover and
+ * all later ones that need a page are refused.  Writes
+ *   q_start [n_requests + 1]  first row of each request's new tokens (clamped to n_tokens)
+ *   kv_len [n_requests]       cached + new, 0 for a refused request
+ *   slots, positions [n_tokens]  page * page_size + offset (-1: no slot) and the token's
+ *                             position in its request (-1 past the last token)
+ *   status [n_requests]       0 or TLX_PAGED_*
+ *   held_out, n_free_out      the state after the call; they may be held_in / n_free_in
+ *                             themselves (the free stack is not written).
+ * The workspace (tlx_paged_plan_workspace_bytes, zeroed once) is left zeroed. */
+#define TLX_PAGED_NO_PAGES 1
+#define TLX_PAGED_TABLE_FULL 2   /* more pages than the table is wide */
+#define TLX_PAGED_BAD_LENGTH 3   /* a negative length, or rows past n_tokens */
+size_t tlx_paged_plan_workspace_bytes(void);
+int tlx_paged_plan(const int32_t* cached_len, const int32_t* new_len, int n_requests, int page_size,
+                   int32_t* block_table, int64_t table_stride, int table_width, const int32_t* held_in,
+                   int32_t* held_out, const int32_t* free_pages, int64_t pages, const int32_t* n_free_in,
+                   int32_t* n_free_out, int n_tokens, int32_t* q_start, int32_t* kv_len, int32_t* slots,
+                   int32_t* positions, int32_t* status, void* ws, size_t ws_bytes, void* stream);
+/* the pages of every request with done[b] != 0 go back on the free stack (request order,
+ * then table order); its table entries become -1 and held[b] 0 */
+int tlx_paged_release(const int32_t* done, int n_requests, int32_t* block_table, int64_t table_stride, int table_width,
+                      int32_t* held, int32_t* free_pages, int64_t pages, int32_t* n_free, void* stream);
+
+/* Rows k, v [n_tokens][kv_heads][head_dim] (fp16, bf16 or fp32; token and head strides in
+ * elements, 16-byte multiples) into their slots; a slot outside the pool is skipped.  A
+ * 16-bit cache takes rows of its own type (copied) or fp32 (rounded once).  TLX_DT_Q8
+ * quantises per 32 dims as tlx_attn_pre does: scale fp16(max|x| / 127) (1e-8, which is 0
+ * in fp16, for an all-zero group), code rint(clamp(x / scale, +-127)) + 128. */
+int tlx_paged_append(const tlx_paged_kv* cache, const void* k, const void* v, int x_dtype, int64_t k_tok_stride,
+                     int64_t k_head_stride, int64_t v_tok_stride, int64_t v_head_stride, const int32_t* slots,
+                     int n_tokens, void* stream);
+
+/* Attention of each request's new tokens over its paged cache (its new rows appended
+ * first).  Row t of the n = q_start[b + 1] - q_start[b] new tokens of request b sees the
+ * keys j <= kv_len[b] - n + t:
+ *   out[q_start[b] + t][h] = softmax_j(scale * q . k_j) v_j  (* sigmoid(gate), if given)
+ * with query head h on KV head h / (heads / kv_heads), heads / kv_heads <= 128.  A row
+ * that sees no key (kv_len 0, say) gives 0; what the pages hold past kv_len is never used.
+ * q, gate and out are [n_tokens][heads][head_dim] of one dtype (fp16 or bf16), token and
+ * head strides in elements, 16-byte multiples.  fp16 q reads fp16 and TLX_DT_Q8 caches,
+ * bf16 q bf16 caches.  max_new: no request has more new tokens (rows past it are not
+ * written); n_tokens is always a valid bound.  Softmax statistics and sums are fp32, the
+ * probabilities are rounded to the dtype of q for the product with v.  Rows past
+ * q_start[n_requests] are not written.  Results do not depend on the order in which the
+ * device runs the work.
+ * Workspace: tlx_paged_attention_workspace_bytes, 256-byte aligned, zeroed once; the first
+ * word holds the error bits of bounded waits (tlx_workspace_error). */
+size_t tlx_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim);
+int tlx_paged_attention(const tlx_paged_kv* cache, const int32_t* block_table, int64_t table_stride, int table_width,
+                        const int32_t* q_start, const int32_t* kv_len, int n_requests, const void* q, int q_dtype,
+                        int64_t q_tok_stride, int64_t q_head_stride, int heads, int n_tokens, int max_new, float scale,
+                        const void* gate, int64_t gate_tok_stride, int64_t gate_head_stride, void* out,
+                        int64_t out_tok_stride, int64_t out_head_stride, void* ws, size_t ws_bytes, void* stream);
+
+/* h = x + residual, y = h * rsqrt(mean(h^2) + eps) * weight, and y in int8 with one scale
+ * per (token, 128-k chunk): s = max(max|y|, 1e-6) * (1/127), xq = clamp(rint(y / s)), the
+ * token format tlx_prefill_w4a8_gate_up reads (tlx_act_quant_q8 quantises fp16 tokens by
+ * the same rule).  x is fp16, bf16 or fp32; residual (NULL: h = x) and h_out (NULL: not
+ * wanted; may be the residual itself) share r_dtype; weight is fp32.  h, the mean and y
+ * stay in fp32; h is rounded once when it is stored.  rs (optional) receives the chunk
+ * sums.  k % 128 == 0, k <= 32768; rows are 16-byte aligned (xq: 8). */
+int tlx_add_rms_norm_q8(const void* x, int x_dtype, int64_t ldx, const void* residual, int r_dtype, int64_t ldr,
+                        const float* weight, float eps, int m, int64_t k, void* h_out, int64_t ldh, int8_t* xq,
+                        int64_t ldq, float* sx, int32_t* rs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,7 +13,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("TLX_LIB", os.path.join(_HERE, "libtlx_b200.so"))
 
 TLX_Q8_0, TLX_Q4_K, TLX_Q5_K, TLX_Q6_K, TLX_IQ3_XXS, TLX_IQ4_XS = 8, 12, 13, 14, 18, 23
-TLX_DT_F32, TLX_DT_F16, TLX_DT_BF16, TLX_DT_IMAGE = 0, 1, 30, 100
+TLX_DT_F32, TLX_DT_F16, TLX_DT_BF16, TLX_DT_IMAGE, TLX_DT_Q8 = 0, 1, 30, 100, 102
 MODE_STORE, MODE_GATE_UP, MODE_ARGMAX = 0, 1, 2
 QTYPES = {"q6_k": TLX_Q6_K, "iq3_xxs": TLX_IQ3_XXS, "iq4_xs": TLX_IQ4_XS, "q4_k": TLX_Q4_K, "q5_k": TLX_Q5_K,
           "q8_0": TLX_Q8_0}
@@ -27,6 +27,16 @@ _lock = threading.Lock()
 _lib = None
 
 c_i64, c_int, c_size, c_vp, c_u32p = ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_void_p
+c_f32 = ctypes.c_float
+
+
+class PagedKV(ctypes.Structure):
+    """tlx_paged_kv: the pool of K / V pages a call reads or writes (strides: page, head, slot)."""
+
+    _fields_ = [("k", c_vp), ("v", c_vp), ("k_scale", c_vp), ("v_scale", c_vp), ("k_stride", c_i64 * 3),
+                ("v_stride", c_i64 * 3), ("ks_stride", c_i64 * 3), ("vs_stride", c_i64 * 3), ("pages", c_i64),
+                ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("dtype", ctypes.c_int32)]
 
 _SIGS = {
     "tlx_error_string": (ctypes.c_char_p, [c_int]),
@@ -104,6 +114,16 @@ _SIGS = {
     "tlx_prefill_gemm": (c_int, [c_int, c_vp, c_vp, c_vp, c_int, c_i64, c_int, c_i64, c_i64, c_vp, c_i64, c_vp,
                                  c_size, c_vp]),
     "tlx_act_quant_q8": (c_int, [c_vp, c_i64, c_int, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp]),
+    "tlx_paged_plan_workspace_bytes": (c_size, []),
+    "tlx_paged_plan": (c_int, [c_vp, c_vp, c_int, c_int, c_vp, c_i64, c_int, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_int,
+                               c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_size, c_vp]),
+    "tlx_paged_release": (c_int, [c_vp, c_int, c_vp, c_i64, c_int, c_vp, c_vp, c_i64, c_vp, c_vp]),
+    "tlx_paged_append": (c_int, [c_vp, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_vp, c_int, c_vp]),
+    "tlx_paged_attention_workspace_bytes": (c_size, [c_int, c_int, c_int]),
+    "tlx_paged_attention": (c_int, [c_vp, c_vp, c_i64, c_int, c_vp, c_vp, c_int, c_vp, c_int, c_i64, c_i64, c_int, c_int,
+                                    c_int, c_f32, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_size, c_vp]),
+    "tlx_add_rms_norm_q8": (c_int, [c_vp, c_int, c_i64, c_vp, c_int, c_i64, c_vp, c_f32, c_int, c_i64, c_vp, c_i64,
+                                    c_vp, c_i64, c_vp, c_vp, c_vp]),
     "tlx_prefill_w4a8_gate_up": (c_int, [c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_int, c_i64, c_i64, c_vp, c_i64,
                                          c_vp, c_size, c_vp]),
 }

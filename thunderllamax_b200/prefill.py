@@ -156,6 +156,45 @@ def w4a8_gate_up(w_gate: torch.Tensor, w_up: torch.Tensor, xq: torch.Tensor, sx:
     return act
 
 
+def add_rms_norm_q8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
+                    out: torch.Tensor = None, xq: torch.Tensor = None, sx: torch.Tensor = None,
+                    rs: torch.Tensor = None):
+    """h = x + residual, y = rms_norm(h) * weight in int8 -> (h in the residual's dtype, xq int8 [m, k],
+    sx fp32 [m, k/128]): the tokens w4a8_gate_up reads.  x and residual are fp16, bf16 or fp32
+    [tokens, k] rows, weight fp32 [k]; residual None: h = x; out may be the residual itself; rs (optional,
+    int32 [m, k/128]) receives the chunk sums."""
+    ops.require_device()
+    if x.dim() != 2 or x.stride(1) != 1 or x.dtype not in ops._DT:
+        raise TLXError("x must be a row-major fp16, bf16 or fp32 [tokens, k] tensor")
+    m, k = x.shape
+    if residual is not None and (residual.shape != x.shape or residual.stride(1) != 1 or
+                                 residual.dtype not in ops._DT or residual.device != x.device):
+        raise TLXError("residual must be a row-major fp16, bf16 or fp32 tensor of x's shape")
+    if weight.dtype != torch.float32 or weight.numel() != k or not weight.is_contiguous() or weight.device != x.device:
+        raise TLXError("weight must be a contiguous fp32 [k] tensor")
+    h_dtype = x.dtype if residual is None else residual.dtype
+    if out is None:
+        out = torch.empty((m, k), dtype=h_dtype, device=x.device)
+    if xq is None:
+        xq = torch.empty((m, k), dtype=torch.int8, device=x.device)
+    if sx is None:
+        sx = torch.empty((m, k // 128), dtype=torch.float32, device=x.device)
+    if out.dtype != h_dtype or out.shape != x.shape or out.stride(1) != 1:
+        raise TLXError("out must be a row-major tensor of the residual's dtype and shape")
+    if xq.dtype != torch.int8 or xq.shape != x.shape or xq.stride(1) != 1:
+        raise TLXError("xq must be a row-major int8 [tokens, k] tensor")
+    _check_chunk_table(sx, torch.float32, m, k, "sx")
+    if rs is not None:
+        _check_chunk_table(rs, torch.int32, m, k, "rs")
+    rc = _lib.lib().tlx_add_rms_norm_q8(x.data_ptr(), ops._DT[x.dtype], x.stride(0),
+                                        None if residual is None else residual.data_ptr(), ops._DT[h_dtype],
+                                        0 if residual is None else residual.stride(0), weight.data_ptr(), eps, m, k,
+                                        out.data_ptr(), out.stride(0), xq.data_ptr(), xq.stride(0), sx.data_ptr(),
+                                        None if rs is None else rs.data_ptr(), ops._stream(x))
+    check(rc, "add_rms_norm_q8")
+    return out, xq, sx
+
+
 class PrefillFFN:
     """The config-5 FFN on one GPU: gate/up (+SiLU) then down, two launches (+ the
     bf16 -> fp16 token staging)."""
