@@ -364,6 +364,18 @@ def test_attention_many_requests(hd, cache):
     Batch(new, kv, 8, 2, hd, cache, 16, seed=1).check()
 
 
+def test_attention_reused_workspace():
+    # one workspace, changing lengths: nothing of an earlier call is left in a later one
+    attn = paged.PagedAttention(8, 2, 128)
+    attn.ws.buf[256:].fill_(0xFF)
+    for i, (new, kv) in enumerate([([1, 1], [900, 64]), ([1, 1], [70, 65]), ([40, 2], [900, 300]), ([1, 1], [129, 1]),
+                                   ([3, 33], [66, 500]), ([1, 1], [65, 2000])]):
+        b = Batch(new, kv, 8, 2, 128, F16, 16, seed=i)
+        got = attn(b.store, b.table, b.q_start, b.kv_len, b.q)
+        ref, tol = b.reference()
+        assert ((got.double() - ref).abs() <= tol).all(), i
+
+
 def test_attention_peaked_scores():
     # one key dominates each row, and the running maximum keeps growing along the keys
     for hd, cache, n in ((256, F16, 1), (128, BF16, 70), (64, F16, 300)):
