@@ -12,10 +12,11 @@
 // rows form (paged_rows_kernel)   requests with at most 16 query rows per KV head (single
 //   tokens, a few drafts): bound by the cache's bytes, so a warp-level matrix product on
 //   16 rows is enough and the decoded keys never leave registers.
-// simple form                     the rest.
+// tiles form (paged_tiles_kernel)  the rest: tcgen05 on tiles of 128 query rows.
 #include <algorithm>
 
 #include "paged.cuh"
+#include "tcgen05.cuh"
 
 namespace tlx {
 namespace {
@@ -42,7 +43,7 @@ struct AttnArgs {
   int rows_limit;        // requests with 1 .. rows_limit query rows per KV head: the rows form
   float* part;           // [2 CTAs][rows][head_dim] unnormalised rows of split items
   float2* ml;            // [2 CTAs][rows] (max, sum)
-  int4* desc;            // split items: {slot of the first piece, last CTA, request, KV head}
+  int4* desc;            // split items: {slot of the first piece, last CTA, request << 10 | KV head, tile}
   int by_item;           // desc is indexed by item (request * kv_heads + head), else by first CTA
 };
 
@@ -69,7 +70,7 @@ __device__ __forceinline__ Req get_req(const AttnArgs& a, int b) {
 // keys is one unit, which writes zeros)
 template <int KT>
 __device__ __forceinline__ int rows_units(const AttnArgs& a, const Req& r) {
-  if (r.n < 1 || r.n * a.group > a.rows_limit) return 0;
+  if (r.n < 1 || r.n * static_cast<int64_t>(a.group) > a.rows_limit) return 0;
   return max(1, (r.keys + KT - 1) / KT) * a.c.kv_heads;
 }
 
@@ -82,7 +83,8 @@ __device__ __forceinline__ int range_of(int64_t units, int64_t u, int ctas) {
 }
 
 // Total units and the request (with the unit inside it) at which this CTA's range starts.
-// Every thread of the block calls it; THREADS = blockDim.x.
+// Every thread of the block calls it; THREADS = blockDim.x; scratch: 8-byte aligned shared
+// memory of THREADS / 4 + 16 bytes, free again after the block's next barrier.
 struct Start {
   int64_t units, u0, u1;
   int64_t local;   // unit inside request b
@@ -90,10 +92,10 @@ struct Start {
   int ctas;        // CTAs that have a unit: an item's pieces are consecutive ones
 };
 template <int THREADS, typename F>
-__device__ __forceinline__ Start find_start(const AttnArgs& a, F units_of) {
-  __shared__ int64_t tot[THREADS / 32];
-  __shared__ int64_t s_local;
-  __shared__ int s_b;
+__device__ __forceinline__ Start find_start(const AttnArgs& a, void* scratch, F units_of) {
+  volatile int64_t* tot = static_cast<int64_t*>(scratch);
+  volatile int64_t& s_local = tot[THREADS / 32];
+  volatile int64_t& s_b = tot[THREADS / 32 + 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int64_t sum = 0;
   for (int b = tid; b < a.n_req; b += THREADS) sum += units_of(b);
@@ -144,20 +146,9 @@ __device__ __forceinline__ Start find_start(const AttnArgs& a, F units_of) {
     }
   }
   __syncthreads();
-  s.b = s_b;
+  s.b = static_cast<int>(s_b);
   s.local = s_local;
   return s;
-}
-
-template <bool BF>
-__device__ __forceinline__ float up16(uint16_t v) {
-  if constexpr (BF) return __uint_as_float(static_cast<uint32_t>(v) << 16);
-  else return __half2float(__ushort_as_half(v));
-}
-template <bool BF>
-__device__ __forceinline__ uint16_t down16(float v) {
-  if constexpr (BF) return __bfloat16_as_ushort(__float2bfloat16(v));
-  else return __half_as_ushort(__float2half(v));
 }
 
 // ------------------------------------------------------------------ rows form
@@ -212,12 +203,6 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&x)[4], uin
   else
     mma16816(d, x, b0, b1);
 }
-// 2^x (ex2.approx: relative error about 2^-22; 2^-inf = 0)
-__device__ __forceinline__ float pow2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-  return y;
-}
 template <bool BF>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if constexpr (BF) {
@@ -244,7 +229,7 @@ __device__ __forceinline__ bool bad16(uint32_t w) {
 }
 
 template <int CT, int HD>
-__global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel(const __grid_constant__ AttnArgs a) {
   using C = RowsCfg<CT, HD>;
   constexpr bool BF = CT == CT_BF16, Q8 = C::kQ8;
   constexpr int KT = C::kKeys, KW = KT / 4, NB = KW / 8;   // keys of a unit, of a warp, its 8-key blocks
@@ -260,7 +245,7 @@ __global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
 
   griddep_launch_dependents();
-  const Start st = find_start<128>(a, [&](int b) { return static_cast<int64_t>(rows_units<KT>(a, get_req(a, b))); });
+  const Start st = find_start<128>(a, psm, [&](int b) { return static_cast<int64_t>(rows_units<KT>(a, get_req(a, b))); });
   if (!a.by_item && tid == 0) a.desc[blockIdx.x] = make_int4(-1, -1, 0, 0);
   const int n_units = static_cast<int>(st.u1 - st.u0);
   if (n_units == 0) return;
@@ -452,15 +437,15 @@ __global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel
       n1 = fmaxf(n1, smax[w * 16 + g + 8]);
     }
     const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;
-    const float f0 = pow2(m0 - b0), f1 = pow2(m1 - b1);   // 0 for the first unit
+    const float f0 = ex2_approx(m0 - b0), f1 = ex2_approx(m1 - b1);   // 0 for the first unit
     m0 = n0;
     m1 = n1;
     l0 *= f0;
     l1 *= f1;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const uint32_t p0 = pack2<BF>(pow2(s[nb][0] - b0), pow2(s[nb][1] - b0));
-      const uint32_t p1 = pack2<BF>(pow2(s[nb][2] - b1), pow2(s[nb][3] - b1));
+      const uint32_t p0 = pack2<BF>(ex2_approx(s[nb][0] - b0), ex2_approx(s[nb][1] - b0));
+      const uint32_t p1 = pack2<BF>(ex2_approx(s[nb][2] - b1), ex2_approx(s[nb][3] - b1));
       // the sum is taken over the rounded probabilities: what rounding does to all of a
       // row's weights alike cancels in the quotient
       const float2 r0 = unpack2<BF>(p0), r1 = unpack2<BF>(p1);
@@ -583,7 +568,7 @@ __global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel
       if (tid == 0) {
         const int64_t item = static_cast<int64_t>(at.b) * a.c.kv_heads + at.head;
         if (begin >= st.u0) {   // the item starts here: where its pieces are, if it is split
-          const int4 d = make_int4(whole ? -1 : slot, whole ? -1 : range_of(st.units, end - 1, st.ctas), at.b, at.head);
+          const int4 d = make_int4(whole ? -1 : slot, whole ? -1 : range_of(st.units, end - 1, st.ctas), at.b << 10 | at.head, 0);
           if (a.by_item) a.desc[item] = d;
           else if (!whole) a.desc[blockIdx.x] = d;
         }
@@ -641,33 +626,774 @@ __global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel
   }
 }
 
+// ----------------------------------------------------------------- tiles form
+// The 128 rows of a tensor-core tile are the query heads of one KV head times as many
+// tokens as fit (row = token * group + head), so every key read serves the whole group.
+// A CTA walks its units (64 keys of one item) on tcgen05:
+//   S(i) = Q K_i^T   M = 128, N = 64, K = head_dim; Q in tensor memory (head_dim 256) or
+//                    shared memory, S double-buffered in tensor memory
+//   O += P(i) V_i    M = 128, N = head_dim, K = 64; V is the MN-major operand as it lies
+//                    in the cache, P (16 bit) in shared memory, double-buffered
+//   warps 0..3   softmax, one thread per row; O is rescaled (in tensor memory) only when a
+//                row's maximum grows by more than 2^8, which keeps P in range
+//   warp 4       one thread issues the MMAs, S(i + 1) ahead of O += P(i) V(i)
+//   warps 5..    K and V halves of the units into a ring, in the order the MMAs read them
+// Every wait is bounded: a timeout raises the error word, all roles leave, issued MMAs
+// and copies are drained and tensor memory is freed.
+__device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t parity) {
+  const bool ok = tc_wait(b, parity);
+  __syncwarp();   // what follows is for the whole warp
+  return ok;
+}
+
+template <int CT, int HD>
+struct TilesCfg {
+  static constexpr bool kQ8 = CT == CT_Q8;
+  static constexpr int kKeys = 64;
+  static constexpr int kHalf = kKeys * HD * 2;                  // bytes of a K or V half
+  static constexpr bool kQTmem = HD == 256;
+  static constexpr int kQBytes = kQTmem ? 0 : 128 * HD * 2;
+  static constexpr int kPBytes = 128 * kKeys * 2;
+  static constexpr int kPBufs = HD == 128 ? 1 : 2;
+  static constexpr int kRing = HD == 64 ? 6 : HD == 128 ? 4 : 6;
+  static constexpr int kProducers = HD == 256 ? 7 : 3;          // warps
+  static constexpr int kThreads = 32 * (5 + kProducers);
+  static constexpr int kCtas = HD == 256 ? 1 : 2;               // on an SM
+  static constexpr int kOffP = kRing * kHalf;
+  static constexpr int kOffQ = kOffP + kPBufs * kPBytes;
+  static constexpr int kOffBar = kOffQ + kQBytes;
+  static constexpr int kSmem = kOffBar + 512;
+  static constexpr uint32_t kTmem = HD == 256 ? 512 : 256;
+  static constexpr uint32_t kColS = 0, kColO = 128;
+  static constexpr uint32_t kColQ = kQTmem ? 384 : 0;
+  static constexpr uint32_t kFmt = CT == CT_BF16 ? (1u << 7) | (1u << 10) : 0u;   // A, B bf16
+  static constexpr uint32_t kIdescQK = (1u << 4) | kFmt | (64u >> 3) << 17 | (128u >> 4) << 24;
+  static constexpr uint32_t kIdescPV = (1u << 4) | kFmt | (1u << 16) | static_cast<uint32_t>(HD >> 3) << 17 | (128u >> 4) << 24;
+};
+
+// sum over i < n of floor((a i + b) / m): the Euclid-like recursion, as a loop
+__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+  int64_t s = 0;
+  while (n > 0) {
+    if (a >= m) {
+      s += (n - 1) * n / 2 * (a / m);
+      a %= m;
+    }
+    if (b >= m) {
+      s += n * (b / m);
+      b %= m;
+    }
+    const int64_t y = a * n + b;
+    if (y < m) break;
+    n = y / m;
+    b = y % m;
+    const int64_t t = m;
+    m = a;
+    a = t;
+  }
+  return s;
+}
+
+__device__ __forceinline__ int tile_tokens(const AttnArgs& a) { return 128 / a.group; }
+__device__ __forceinline__ int tile_count(const AttnArgs& a, const Req& r) {
+  if (r.n < 1 || r.n * static_cast<int64_t>(a.group) <= a.rows_limit) return 0;
+  return (r.n + tile_tokens(a) - 1) / tile_tokens(a);
+}
+// keys that the last token of the tile sees
+__device__ __forceinline__ int tile_keys(const AttnArgs& a, const Req& r, int tile) {
+  const int64_t last = min(static_cast<int64_t>(tile + 1) * tile_tokens(a), static_cast<int64_t>(r.n));
+  return static_cast<int>(min(max(static_cast<int64_t>(r.kv) - r.n_all + last, static_cast<int64_t>(0)),
+                              static_cast<int64_t>(r.keys)));
+}
+__device__ __forceinline__ int tile_units(const AttnArgs& a, const Req& r, int tile) {
+  return max(1, (tile_keys(a, r, tile) + 63) >> 6);
+}
+// units of one KV head in the tiles before `tile`
+__device__ __forceinline__ int64_t units_before(const AttnArgs& a, const Req& r, int tile) {
+  const int64_t tt = tile_tokens(a), c = static_cast<int64_t>(r.kv) - r.n_all;
+  const int full = min(tile, r.n / static_cast<int>(tt));   // tiles with all their tokens
+  int64_t s = 0;
+  int i = 0;
+  if (c >= 0 && r.keys == r.kv) {   // ceil((c + (i + 1) tt) / 64), at least 1 since tt >= 1
+    s = floor_sum(full, 64, tt, c + tt + 63);
+    i = full;
+  }
+  for (; i < tile; ++i) s += tile_units(a, r, i);
+  return s;
+}
+
+// The producers replace infinite and NaN values of V by 0 in the units that some rows do
+// not see whole (0 * inf in the product would reach those rows); this adds weight * value
+// of such keys to the rows that do see them.  Called by whole warps with O at rest; the
+// weights are the rounded ones of the product, from P in shared memory.
+template <int CT, int HD>
+__device__ __noinline__ void restore_bad_values(const AttnArgs& a, int b, int head, int k0, int keys, int lim,
+                                                const uint8_t* p_buf, int row, uint32_t o_tmem) {
+  constexpr bool BF = CT == CT_BF16;
+  for (int c = 0; c < HD / 32; ++c) {
+    uint32_t r[32];
+    tc_ld32(o_tmem + c * 32, r);
+    tc_wait_ld();
+    for (int j = 0; j < 64 && k0 + j < keys; ++j) {
+      const int key = k0 + j;
+      const int page = a.table[b * a.table_ld + (key >> a.shift)];
+      if (page < 0 || page >= a.c.pages) continue;
+      const int64_t in = key & (a.c.page_size - 1);
+      const int64_t at = page * a.c.v_stride[0] + head * a.c.v_stride[1] + in * a.c.v_stride[2] + c * 32;
+      const float p = unpack2<BF>(*reinterpret_cast<const uint16_t*>(p_buf + sw128(row, j >> 3) + (j & 7) * 2)).x;
+#pragma unroll
+      for (int x = 0; x < 32; ++x) {
+        uint32_t v;
+        if constexpr (CT == CT_Q8) {
+          const uint32_t s = static_cast<const uint16_t*>(
+              a.c.v_scale)[page * a.c.vs_stride[0] + head * a.c.vs_stride[1] + in * a.c.vs_stride[2] + c];
+          v = dq2(static_cast<const uint8_t*>(a.c.v)[at + x], 0x4040u, s | s << 16) & 0xFFFFu;
+        } else {
+          v = static_cast<const uint16_t*>(a.c.v)[at + x];
+        }
+        if (bad16<BF>(v) && key < lim) r[x] = __float_as_uint(__uint_as_float(r[x]) + p * unpack2<BF>(v).x);
+      }
+    }
+    __syncwarp();
+    tc_st32(o_tmem + c * 32, r);
+    tc_wait_st();
+  }
+}
+
+template <int CT, int HD>
+__global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::kCtas)
+    paged_tiles_kernel(const __grid_constant__ AttnArgs a, uint32_t* err) {
+  using C = TilesCfg<CT, HD>;
+  constexpr bool BF = CT == CT_BF16, Q8 = C::kQ8;
+  static_assert(C::kColO + HD + (C::kQTmem ? C::kColQ - 384 + HD / 2 : 0) <= C::kTmem, "tensor memory");
+  constexpr int NP = C::kProducers, RING = C::kRing, PB = C::kPBufs;
+  extern __shared__ __align__(1024) uint8_t sm_tiles[];
+  uint8_t* const sm = sm_tiles;
+  uint64_t* bar = reinterpret_cast<uint64_t*>(sm + C::kOffBar);
+  uint64_t* full = bar;                 // [RING] producers -> MMA
+  uint64_t* empty = full + RING;        // [RING] MMA -> producers
+  uint64_t* s_full = empty + RING;      // [2] MMA -> softmax
+  uint64_t* s_free = s_full + 2;        // [2] softmax -> MMA
+  uint64_t* p_full = s_free + 2;        // [2] softmax -> MMA
+  uint64_t* pv_done = p_full + 2;       // [2] MMA -> softmax
+  uint64_t* q_full = pv_done + 2;       // softmax -> MMA: Q of the next item is in
+  uint64_t* o_free = q_full + 1;        // softmax -> MMA: O of the last item is read
+  uint64_t* done = o_free + 1;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(done + 1);
+  volatile uint32_t* abort_flag = tmem_holder + 1;
+  // [8] by unit: unit + 1 if the producers took a bad value out of its V (they are fewer
+  // than 8 units ahead of the softmax)
+  volatile int* bad = reinterpret_cast<int*>(tmem_holder + 2);
+  struct First {
+    int tile, head, u;
+  };
+  First* first_at = reinterpret_cast<First*>(tmem_holder + 10);
+  static_assert((2 * RING + 11) * 8 + 10 * 4 + sizeof(First) <= 512, "barrier area");
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  griddep_launch_dependents();
+  const Start st = find_start<C::kThreads>(a, sm + C::kOffP, [&](int b) -> int64_t {
+    const Req r = get_req(a, b);
+    const int tiles = tile_count(a, r);
+    return tiles ? units_before(a, r, tiles) * a.c.kv_heads : 0;
+  });
+  if (tid == 0) a.desc[blockIdx.x] = make_int4(-1, -1, 0, 0);
+  const int n = static_cast<int>(st.u1 - st.u0);
+  if (n == 0) return;
+  const uint32_t sbase = smem_u32(sm);
+  if (sbase & 1023u) {   // the descriptors need the swizzle atoms' alignment
+    if (tid == 0) atomicOr(err, ERR_BAD_PARAM);
+    return;
+  }
+  if (warp == 0) {   // the tile, head and unit at which the range starts: a 32-way search
+    const Req r = get_req(a, st.b);
+    int lo = 0, hi = tile_count(a, r);   // units_before(lo) * heads <= local < units_before(hi) * heads
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 31) / 32, t = min(lo + lane * step, hi);
+      const bool le = t < hi && units_before(a, r, t) * a.c.kv_heads <= st.local;
+      const int k = 31 - __clz(__ballot_sync(0xffffffffu, le));   // lane 0 always holds
+      const int nlo = lo + k * step;
+      hi = min(hi, nlo + step);
+      lo = nlo;
+    }
+    if (lane == 0) {
+      const int64_t rest = st.local - units_before(a, r, lo) * a.c.kv_heads;
+      const int of = tile_units(a, r, lo);
+      *first_at = First{lo, static_cast<int>(rest / of), static_cast<int>(rest % of)};
+    }
+  }
+  if (tid == 0) {
+    for (int i = 0; i < RING; ++i) {
+      mbar_init(&full[i], NP);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 8; ++i) bad[i] = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_free[i], 4);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&pv_done[i], 1);
+    }
+    mbar_init(q_full, 4);
+    mbar_init(o_free, 4);
+    mbar_init(done, 1);
+    *abort_flag = 0u;
+    mbar_fence_init();
+  }
+  if (warp == 4) tc_alloc(tmem_holder, C::kTmem);
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = *tmem_holder;
+  auto fail = [&]() {
+    atomicOr(err, ERR_MBAR_TIMEOUT);
+    *abort_flag = 1u;
+  };
+
+  struct Pos {
+    int b, tile, head, u, of, tiles;
+    Req r;
+  };
+  Pos at;
+  at.b = st.b;
+  at.r = get_req(a, st.b);
+  at.tiles = tile_count(a, at.r);
+  at.tile = first_at->tile;
+  at.head = first_at->head;
+  at.u = first_at->u;
+  at.of = tile_units(a, at.r, at.tile);
+  // the next item (not called past the last unit of the launch)
+  auto next_item = [&](Pos& p) {
+    p.u = 0;
+    if (++p.head == a.c.kv_heads) {
+      p.head = 0;
+      if (++p.tile == p.tiles) {
+        p.tile = 0;
+        do {
+          if (++p.b >= a.n_req) return;
+          p.r = get_req(a, p.b);
+          p.tiles = tile_count(a, p.r);
+        } while (p.tiles == 0);
+      }
+      p.of = tile_units(a, p.r, p.tile);
+    }
+  };
+
+  if (warp == 4) {
+    // --------------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      int h = 0;          // ring halves consumed
+      int item = 0, left = min(at.of - at.u, n);   // units left of the current item
+      auto issue_qk = [&](int i, bool starts, int it) -> bool {
+        const int b = i & 1, slot = h % RING;
+        if (starts && !tc_wait(q_full, it & 1)) return false;
+        if (!tc_wait(&full[slot], (h / RING) & 1) || !tc_wait(&s_free[b], ((i >> 1) & 1) ^ 1)) return false;
+        tc_after();
+        const uint32_t kb = sbase + slot * C::kHalf;
+#pragma unroll
+        for (int s = 0; s < HD / 16; ++s) {
+          const uint64_t bd = sw128_desc(kb + (s >> 2) * 8192 + (s & 3) * 32);
+          if constexpr (C::kQTmem)
+            tc_mma_ts(tmem + C::kColS + b * 64, tmem + C::kColQ + s * 8, bd, C::kIdescQK, s > 0 ? 1u : 0u);
+          else
+            tc_mma(tmem + C::kColS + b * 64, sw128_desc(sbase + C::kOffQ + (s >> 2) * 16384 + (s & 3) * 32), bd,
+                   C::kIdescQK, s > 0 ? 1u : 0u);
+        }
+        tc_commit(&s_full[b]);
+        tc_commit(&empty[slot]);
+        ++h;
+        return true;
+      };
+      auto issue_pv = [&](int i, bool starts, int it) -> bool {
+        const int slot = h % RING, pb = PB == 2 ? i & 1 : 0;
+        if (starts && it > 0 && !tc_wait(o_free, (it - 1) & 1)) return false;
+        if (!tc_wait(&full[slot], (h / RING) & 1) || !tc_wait(&p_full[i & 1], (i >> 1) & 1)) return false;
+        tc_after();
+        const uint32_t vb = sbase + slot * C::kHalf;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          tc_mma(tmem + C::kColO, sw128_desc(sbase + C::kOffP + pb * C::kPBytes + kk * 32),
+                 sw128_desc_mn(vb + kk * 2048, 8192), C::kIdescPV, (!starts || kk > 0) ? 1u : 0u);
+        tc_commit(&pv_done[i & 1]);
+        tc_commit(&empty[slot]);
+        ++h;
+        return true;
+      };
+      bool ok = issue_qk(0, true, 0), starts = true;
+      for (int i = 0; i < n && ok && !*abort_flag; ++i) {
+        const bool ends = --left == 0;
+        if (!ends && i + 1 < n) ok = issue_qk(i + 1, false, item);
+        ok = ok && issue_pv(i, starts, item);
+        starts = ends;
+        if (ends && i + 1 < n) {
+          next_item(at);
+          left = at.of;
+          ++item;
+          ok = ok && issue_qk(i + 1, true, item);
+        }
+      }
+      if (!ok) fail();
+      tc_commit(done);   // every issued MMA has completed before tensor memory is released
+      if (!tc_wait(done, 0)) fail();
+    }
+  } else if (warp < 4) {
+    // ----------------------------------------------------------------- softmax
+    const int row = warp * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+    const float sc = a.scale * 1.4426950408889634f;
+    const int tt = tile_tokens(a), t_in = row / a.group, hl = row - t_in * a.group;
+    bool ok = true;
+    auto load_q = [&](const Pos& p) {   // this row of Q (zero past the last row)
+      const int t = p.tile * tt + t_in;
+      const bool valid = t_in < tt && t < p.r.n;
+      const uint4* src = reinterpret_cast<const uint4*>(a.q + static_cast<int64_t>(p.r.q0 + t) * a.q_tok +
+                                                        (p.head * a.group + hl) * a.q_head);
+#pragma unroll 1
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t w[16];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint4 v = valid ? __ldg(src + c * 4 + j) : make_uint4(0u, 0u, 0u, 0u);
+          if constexpr (C::kQTmem) {
+            w[4 * j] = v.x;
+            w[4 * j + 1] = v.y;
+            w[4 * j + 2] = v.z;
+            w[4 * j + 3] = v.w;
+          } else {
+            const int ch = c * 4 + j;
+            *reinterpret_cast<uint4*>(sm + C::kOffQ + (ch >> 3) * 16384 + sw128(row, ch & 7)) = v;
+          }
+        }
+        if constexpr (C::kQTmem) tc_st16(tmem + lanes + C::kColQ + c * 16, w);
+      }
+      if constexpr (C::kQTmem) {
+        tc_wait_st();
+        tc_before();
+      } else {
+        fence_proxy_async_smem();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    };
+    load_q(at);
+    int i = 0;
+    while (i < n && ok && !*abort_flag) {
+      // one item, or this CTA's part of it
+      const int count = min(at.of - at.u, n - i);
+      const int t = at.tile * tt + t_in;
+      const bool valid = t_in < tt && t < at.r.n;
+      const int lim = valid ? max(0, min(at.r.keys, at.r.kv - at.r.n_all + t + 1)) : 0;   // keys < lim
+      const int lim_first = max(0, min(at.r.keys, at.r.kv - at.r.n_all + at.tile * tt + 1));
+      const bool any = __any_sync(0xffffffffu, valid);   // a warp without rows only keeps the barriers going
+      float m_ref = -INFINITY, l_run = 0.f;
+      Pos next = at;
+      for (int k = 0; k < count && ok; ++k, ++i) {
+        const int b = i & 1, pb = PB == 2 ? b : 0;
+        if (!(ok = warp_wait(&s_full[b], (i >> 1) & 1))) break;
+        tc_after();
+        float s[64];
+        if (any) {
+          uint32_t r0[32], r1[32];
+          tc_ld32(tmem + lanes + C::kColS + b * 64, r0);
+          tc_ld32(tmem + lanes + C::kColS + b * 64 + 32, r1);
+          tc_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            s[j] = __uint_as_float(r0[j]) * sc;
+            s[32 + j] = __uint_as_float(r1[j]) * sc;
+          }
+        }
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[b]);
+        const int k0 = (at.u + k) * 64;
+        float off = 0.f;
+        if (any) {
+          const int rem = lim - k0;
+          if (__any_sync(0xffffffffu, rem < 64)) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) s[j] = j < rem ? s[j] : -INFINITY;
+          }
+          float mx[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) mx[j] = s[j];
+#pragma unroll
+          for (int j = 8; j < 64; ++j) mx[j & 7] = fmaxf(mx[j & 7], s[j]);
+          const float mt = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
+                                 fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
+          const bool grows = mt > m_ref + 8.f || (m_ref == -INFINITY && mt > -INFINITY);
+          if (__any_sync(0xffffffffu, grows)) {
+            const float m_new = grows ? mt : m_ref;
+            const float cor = m_ref == m_new ? 1.f : ex2_approx(m_ref - m_new);
+            if (k > 0) {
+              if (!(ok = warp_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1))) break;   // O is at rest
+              tc_after();
+              l_run *= cor;
+#pragma unroll 1
+              for (int c = 0; c < HD / 32; ++c) {
+                uint32_t r[32];
+                tc_ld32(tmem + lanes + C::kColO + c * 32, r);
+                tc_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * cor);
+                tc_st32(tmem + lanes + C::kColO + c * 32, r);
+              }
+              tc_wait_st();
+            }
+            m_ref = m_new;
+          }
+          off = m_ref == -INFINITY ? 0.f : m_ref;
+        }
+        // the P buffer is free once the product that read it is done
+        if (i >= PB && !(ok = warp_wait(&pv_done[(i - PB) & 1], ((i - PB) >> 1) & 1))) break;
+        if (any) {
+          float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              w[j] = pack2<BF>(ex2_approx(s[8 * c + 2 * j] - off), ex2_approx(s[8 * c + 2 * j + 1] - off));
+              const float2 p = unpack2<BF>(w[j]);   // the rounded weights are summed: see the rows form
+              sums[j] += p.x + p.y;
+            }
+            *reinterpret_cast<uint4*>(sm + C::kOffP + pb * C::kPBytes + sw128(row, c)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          l_run += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        }
+        fence_proxy_async_smem();
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[b]);
+        // Q of the next item may follow once every S of this one is read
+        if (k + 1 == count && i + 1 < n) {
+          next_item(next);
+          load_q(next);
+        }
+        // bad values that the producers took out of V, for the rows that see them
+        if (any && lim_first < min(k0 + 64, at.r.keys)) {
+          if (!(ok = warp_wait(&pv_done[b], (i >> 1) & 1))) break;
+          tc_after();
+          if (bad[i & 7] == i + 1)
+            restore_bad_values<CT, HD>(a, at.b, at.head, k0, at.r.keys, lim, sm + C::kOffP + pb * C::kPBytes, row,
+                                       tmem + lanes + C::kColO);
+        }
+      }
+      if (!ok) break;
+      // the item's rows, or this part's
+      if (!(ok = warp_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1))) break;
+      tc_after();
+      const int64_t begin = st.u0 + (i - count) - at.u, end = begin + at.of;   // the item's units
+      const bool whole = begin >= st.u0 && end <= st.u1;
+      const int slot = 2 * blockIdx.x + (begin > st.u0 ? 1 : 0);
+      if (tid == 0 && begin >= st.u0 && !whole)
+        a.desc[blockIdx.x] = make_int4(slot, range_of(st.units, end - 1, st.ctas), at.b << 10 | at.head, at.tile);
+      if (any) {
+        const bool sees = lim > 0;
+        const float inv = 1.f / l_run;
+        const int64_t tok = at.r.q0 + t;
+        const int head = at.head * a.group + hl;
+#pragma unroll 1
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t r[32];
+          tc_ld32(tmem + lanes + C::kColO + c * 32, r);
+          tc_wait_ld();
+          if (!valid) continue;
+          if (!whole) {
+            float4* dst = reinterpret_cast<float4*>(a.part + (static_cast<int64_t>(slot) * 128 + row) * HD + c * 32);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              dst[j] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
+                                   __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
+          } else {
+            const uint4* gp = reinterpret_cast<const uint4*>(a.gate + tok * a.g_tok + head * a.g_head + c * 32);
+            uint4* dst = reinterpret_cast<uint4*>(a.out + tok * a.o_tok + head * a.o_head + c * 32);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              float v[8];
+#pragma unroll
+              for (int x = 0; x < 8; ++x) v[x] = sees ? __uint_as_float(r[8 * j + x]) * inv : 0.f;
+              if (a.gate) {
+                const uint4 gv = __ldg(gp + j);
+                const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w};
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                  const float2 y = unpack2<BF>(gw[x]);
+                  v[2 * x] /= 1.f + __expf(-y.x);
+                  v[2 * x + 1] /= 1.f + __expf(-y.y);
+                }
+              }
+              dst[j] = make_uint4(pack2<BF>(v[0], v[1]), pack2<BF>(v[2], v[3]), pack2<BF>(v[4], v[5]), pack2<BF>(v[6], v[7]));
+            }
+          }
+        }
+        if (!whole && valid) a.ml[slot * 128 + row] = make_float2(m_ref, l_run);
+      }
+      tc_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(o_free);
+      at = next;
+    }
+    if (!ok) fail();
+  } else {
+    // --------------------------------------------------------------- producers
+    // The halves in MMA order: K(0), then per unit K(i + 1) and V(i), with V(i) first
+    // where unit i ends an item.  A warp moves every NP-th group of 32 16-byte chunks.
+    const int pw = warp - 5;
+    constexpr int CPK = HD * (Q8 ? 1 : 2) / 16;          // 16-byte chunks of a cached row
+    constexpr int OPS = 64 * CPK / 32;                   // warp operations of a half
+    constexpr int PER = (OPS + NP - 1) / NP;
+    bool ok = true;
+    int h = 0;
+    Pos kp = at, vp = at;    // units of the next K and V halves
+    int ki = 0, vi = 0, kleft = min(at.of - at.u, n), vleft = kleft;
+    auto step = [&](Pos& p, int& idx, int& left) {   // to the next unit
+      ++idx;
+      ++p.u;
+      if (--left == 0 && idx < n) {
+        next_item(p);
+        left = p.of;
+      }
+    };
+    // rows of the half's 64 keys: lane l holds keys l and l + 32
+    struct Rows {
+      int64_t off[2], soff[2];
+      uint32_t ok[2];
+    };
+    auto find_rows = [&](const Pos& p, bool v, Rows& w) {
+      const int64_t* cs = v ? a.c.v_stride : a.c.k_stride;
+      const int64_t* ss = v ? a.c.vs_stride : a.c.ks_stride;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int key = p.u * 64 + x * 32 + lane;
+        w.off[x] = 0;
+        w.soff[x] = 0;
+        bool in_pool = key < p.r.keys;
+        if (in_pool) {
+          const int page = a.table[p.b * a.table_ld + (key >> a.shift)];
+          in_pool = page >= 0 && page < a.c.pages;
+          if (in_pool) {
+            const int64_t in = key & (a.c.page_size - 1);
+            w.off[x] = (page * cs[0] + p.head * cs[1] + in * cs[2]) * (Q8 ? 1 : 2);
+            if constexpr (Q8) w.soff[x] = page * ss[0] + p.head * ss[1] + in * ss[2];
+          }
+        }
+        w.ok[x] = __ballot_sync(0xffffffffu, in_pool);
+      }
+    };
+    // V of a unit that some row of the tile does not see whole: bad values are taken out
+    auto is_edge = [&](const Pos& p) {
+      return max(0, min(p.r.keys, p.r.kv - p.r.n_all + p.tile * tile_tokens(a) + 1)) < min(p.u * 64 + 64, p.r.keys);
+    };
+    const int total = 2 * n;
+    bool k_turn = true;
+    auto after = [&](bool v) {   // order of the halves
+      if (!v) {
+        step(kp, ki, kleft);
+        k_turn = ki == 1 + vi ? (ki < n && vleft != 1) : false;
+      } else {
+        step(vp, vi, vleft);
+        k_turn = ki < n && (ki == vi || vleft != 1);
+      }
+    };
+    if constexpr (!Q8) {
+      constexpr int AHEAD = RING - 2;
+      uint32_t edge_of = 0;             // bit (half % 32): that half needs the check
+      int unit_of[RING];
+      auto finish = [&](int f) {        // half f has landed
+        const int slot = f % RING;
+        if ((edge_of >> (f & 31)) & 1) {
+          uint8_t* hb = sm + slot * C::kHalf;
+          bool any_bad = false;
+          for (int x = 0; x < PER; ++x) {
+            const int op = pw + NP * x;
+            if (op >= OPS) break;
+            const int idx = op * 32 + lane, key = idx / CPK, ch = idx % CPK;
+            uint4* p = reinterpret_cast<uint4*>(hb + (ch >> 3) * 8192 + sw128(key, ch & 7));
+            uint4 v = *p;
+            uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            bool mine = false;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              if (bad16<BF>(w[y] & 0xFFFFu)) {
+                w[y] &= 0xFFFF0000u;
+                mine = true;
+              }
+              if (bad16<BF>(w[y] >> 16)) {
+                w[y] &= 0xFFFFu;
+                mine = true;
+              }
+            }
+            if (mine) {
+              *p = make_uint4(w[0], w[1], w[2], w[3]);
+              any_bad = true;
+            }
+          }
+          if (any_bad) {
+            int u = 0;
+#pragma unroll
+            for (int x = 0; x < RING; ++x)
+              if (x == slot) u = unit_of[x];
+            bad[u & 7] = u + 1;
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[slot]);
+      };
+      for (; h < total && ok && !*abort_flag; ++h) {
+        const int slot = h % RING;
+        const bool v = !k_turn;
+        Rows w;
+        edge_of &= ~(1u << (h & 31));
+        if (v) {
+          find_rows(vp, true, w);
+          if (is_edge(vp)) edge_of |= 1u << (h & 31);
+        } else {
+          find_rows(kp, false, w);
+        }
+#pragma unroll
+        for (int x = 0; x < RING; ++x)
+          if (x == slot) unit_of[x] = v ? vi : ki;
+        if (!(ok = tc_wait(&empty[slot], ((h / RING) & 1) ^ 1))) break;
+        const uint8_t* base = static_cast<const uint8_t*>(v ? a.c.v : a.c.k);
+        const uint32_t hb = sbase + slot * C::kHalf;
+#pragma unroll 8
+        for (int x = 0; x < PER; ++x) {
+          const int op = pw + NP * x;
+          if (op < OPS) {
+            const int idx = op * 32 + lane, key = idx / CPK, ch = idx % CPK;
+            const bool hi = op * 32 / CPK >= 32;   // the same for the warp
+            const int64_t off = __shfl_sync(0xffffffffu, hi ? w.off[1] : w.off[0], key & 31);
+            const bool in_pool = ((hi ? w.ok[1] : w.ok[0]) >> (key & 31)) & 1;
+            cp_async16(hb + (ch >> 3) * 8192 + sw128(key, ch & 7), base + off + ch * 16, in_pool);
+          }
+        }
+        cp_async_commit();
+        after(v);
+        if (h >= AHEAD) {
+          cp_async_wait<AHEAD>();
+          finish(h - AHEAD);
+        }
+      }
+      cp_async_wait<0>();
+      if (ok && !*abort_flag)
+        for (int f = max(0, total - AHEAD); f < total; ++f) finish(f);
+    } else {
+      // codes into registers one half ahead, then fp16(code * scale) into the ring
+      uint4 cur[PER], nxt[PER];
+      uint16_t cs[PER], ns[PER];
+      auto fetch = [&](bool v, uint4 (&q)[PER], uint16_t (&sc)[PER]) {
+        Rows w;
+        if (v) find_rows(vp, true, w);
+        else find_rows(kp, false, w);
+        const uint8_t* base = static_cast<const uint8_t*>(v ? a.c.v : a.c.k);
+        const uint16_t* sb = static_cast<const uint16_t*>(v ? a.c.v_scale : a.c.k_scale);
+#pragma unroll
+        for (int x = 0; x < PER; ++x) {
+          const int op = pw + NP * x;
+          q[x] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+          sc[x] = 0;
+          if (op < OPS) {
+            const int idx = op * 32 + lane, key = idx / CPK, ch = idx % CPK;
+            const bool hi = op * 32 / CPK >= 32;
+            const int64_t off = __shfl_sync(0xffffffffu, hi ? w.off[1] : w.off[0], key & 31);
+            const int64_t so = __shfl_sync(0xffffffffu, hi ? w.soff[1] : w.soff[0], key & 31);
+            if (((hi ? w.ok[1] : w.ok[0]) >> (key & 31)) & 1) {
+              q[x] = __ldg(reinterpret_cast<const uint4*>(base + off + ch * 16));
+              sc[x] = __ldg(sb + so + (ch >> 1));
+            }
+          }
+        }
+      };
+      bool v = !k_turn;
+      fetch(v, nxt, ns);
+      for (; h < total && ok && !*abort_flag; ++h) {
+        const int slot = h % RING;
+        const bool edge = v && is_edge(vp);
+        const int unit = v ? vi : ki;
+#pragma unroll
+        for (int x = 0; x < PER; ++x) {
+          cur[x] = nxt[x];
+          cs[x] = ns[x];
+        }
+        after(v);
+        if (h + 1 < total) {
+          v = !k_turn;
+          fetch(v, nxt, ns);   // in flight while this half is written
+        }
+        if (!(ok = tc_wait(&empty[slot], ((h / RING) & 1) ^ 1))) break;
+        bool any_bad = false;
+#pragma unroll
+        for (int x = 0; x < PER; ++x) {
+          const int op = pw + NP * x;
+          if (op < OPS) {
+            const int idx = op * 32 + lane, key = idx / CPK, ch = idx % CPK;   // 16 dims: chunks 2 ch, 2 ch + 1
+            const uint32_t s2 = cs[x] | static_cast<uint32_t>(cs[x]) << 16;
+            const uint32_t in[4] = {cur[x].x, cur[x].y, cur[x].z, cur[x].w};
+            uint32_t o[8];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              o[2 * y] = dq2(in[y], 0x5140u, s2);
+              o[2 * y + 1] = dq2(in[y], 0x7362u, s2);
+            }
+            if (edge) {
+#pragma unroll
+              for (int y = 0; y < 8; ++y) {
+                if (bad16<false>(o[y] & 0xFFFFu)) {
+                  o[y] &= 0xFFFF0000u;
+                  any_bad = true;
+                }
+                if (bad16<false>(o[y] >> 16)) {
+                  o[y] &= 0xFFFFu;
+                  any_bad = true;
+                }
+              }
+            }
+            uint8_t* hb = sm + slot * C::kHalf + (ch >> 2) * 8192;
+            *reinterpret_cast<uint4*>(hb + sw128(key, (2 * ch) & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<uint4*>(hb + sw128(key, (2 * ch + 1) & 7)) = make_uint4(o[4], o[5], o[6], o[7]);
+          }
+        }
+        if (any_bad) bad[unit & 7] = unit + 1;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[slot]);
+      }
+    }
+    if (!ok) fail();
+  }
+
+  tc_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc_after();
+    tc_dealloc(tmem, C::kTmem);
+  }
+}
+
 // -------------------------------------------------------------------- combine
-// One block per (split item, row).  The pieces' maxima give their weights; groups of
-// threads sum a contiguous share of the pieces each, in piece order, and the groups' sums
-// are added in order, so the result does not depend on when anything ran.
+// A block per split item and row (or every gridDim.y-th row).  The pieces' maxima give
+// their weights; groups of threads sum a contiguous share of the pieces each, in piece
+// order, and the groups' sums are added in order, so the result does not depend on when
+// anything ran.
 template <bool BF, int HD, int ROWS>
-__global__ void __launch_bounds__(256) paged_combine_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constant__ AttnArgs a) {
   constexpr int kLanes = HD / 4, kGroups = 256 / kLanes;
   __shared__ float wgt[kMaxPieces];
   __shared__ float4 acc[256];
   __shared__ float red[8];
   griddep_wait();
-  const int row = blockIdx.y, tid = threadIdx.x;
-  int b = 0, head = 0;
+  const int tid = threadIdx.x;
   if (a.by_item) {   // only the items of this launch have written their entry
-    b = blockIdx.x / a.c.kv_heads;
-    head = blockIdx.x % a.c.kv_heads;
-    const Req r = get_req(a, b);
-    if (r.n < 1 || r.n * a.group > a.rows_limit) return;
+    const Req r = get_req(a, blockIdx.x / a.c.kv_heads);
+    if (r.n < 1 || r.n * static_cast<int64_t>(a.group) > a.rows_limit) return;
   }
-  const int4 d = a.desc[blockIdx.x];   // {slot of the first piece, last CTA, request, KV head}
+  const int4 d = a.desc[blockIdx.x];   // {slot of the first piece, last CTA, request << 10 | KV head, tile}
   if (d.x < 0) return;
-  if (!a.by_item) {
-    b = d.z;
-    head = d.w;
-  }
+  const int b = d.z >> 10, head = d.z & 1023;
   const Req r = get_req(a, b);
-  if (row >= r.n * a.group) return;
+  const int tt = 128 / a.group, t0 = d.w * tt, rows = min(tt, r.n - t0) * a.group;
   const int c0 = d.x >> 1, pieces = min(d.y - c0 + 1, kMaxPieces);
   auto slot_of = [&](int p) { return p == 0 ? d.x : 2 * (c0 + p); };
   auto block_reduce = [&](float v, bool is_max) {
@@ -684,129 +1410,58 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const AttnArgs a) {
     for (int w = 1; w < 8; ++w) v = is_max ? fmaxf(v, red[w]) : v + red[w];
     return v;
   };
-  float m = -INFINITY;
-  for (int p = tid; p < pieces; p += 256) m = fmaxf(m, a.ml[slot_of(p) * ROWS + row].x);
-  m = block_reduce(m, true);
-  const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  for (int p = tid; p < pieces; p += 256) {
-    const float2 x = a.ml[slot_of(p) * ROWS + row];
-    const float w = pow2(x.x - base);
-    wgt[p] = w;
-    l += x.y * w;
-  }
-  l = block_reduce(l, false);   // its barriers also publish wgt
   const int lane = tid % kLanes, grp = tid / kLanes;
   const int p0 = pieces * grp / kGroups, p1 = pieces * (grp + 1) / kGroups;
-  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int row = blockIdx.y; row < rows; row += gridDim.y) {
+    float m = -INFINITY;
+    for (int p = tid; p < pieces; p += 256) m = fmaxf(m, a.ml[slot_of(p) * ROWS + row].x);
+    m = block_reduce(m, true);   // (its barriers also end the last row's use of wgt and acc)
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    for (int p = tid; p < pieces; p += 256) {
+      const float2 x = a.ml[slot_of(p) * ROWS + row];
+      const float w = ex2_approx(x.x - base);
+      wgt[p] = w;
+      l += x.y * w;
+    }
+    l = block_reduce(l, false);   // (its barriers also publish wgt)
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-  for (int p = p0; p < p1; ++p) {
-    const float4 v = *reinterpret_cast<const float4*>(a.part + (static_cast<int64_t>(slot_of(p)) * ROWS + row) * HD + 4 * lane);
-    const float w = wgt[p];
-    s.x = fmaf(v.x, w, s.x);
-    s.y = fmaf(v.y, w, s.y);
-    s.z = fmaf(v.z, w, s.z);
-    s.w = fmaf(v.w, w, s.w);
-  }
-  acc[tid] = s;
-  __syncthreads();
-  if (grp > 0) return;
-  for (int k = 1; k < kGroups; ++k) {
-    const float4 v = acc[k * kLanes + lane];
-    s.x += v.x;
-    s.y += v.y;
-    s.z += v.z;
-    s.w += v.w;
-  }
-  const int t = row / a.group, hq = head * a.group + row - t * a.group;
-  const bool sees = min(r.keys, r.kv - r.n_all + t + 1) > 0;
-  float v[4] = {s.x / l, s.y / l, s.z / l, s.w / l};
-  const int64_t tok = r.q0 + t;
-  if (a.gate) {
-    const uint2 x = *reinterpret_cast<const uint2*>(a.gate + tok * a.g_tok + hq * a.g_head + 4 * lane);
-    const float2 x0 = unpack2<BF>(x.x), x1 = unpack2<BF>(x.y);
-    v[0] /= 1.f + __expf(-x0.x);
-    v[1] /= 1.f + __expf(-x0.y);
-    v[2] /= 1.f + __expf(-x1.x);
-    v[3] /= 1.f + __expf(-x1.y);
-  }
-  if (!sees) v[0] = v[1] = v[2] = v[3] = 0.f;
-  *reinterpret_cast<uint2*>(a.out + tok * a.o_tok + hq * a.o_head + 4 * lane) =
-      make_uint2(pack2<BF>(v[0], v[1]), pack2<BF>(v[2], v[3]));
-}
-
-// ---------------------------------------------------------------- simple form
-template <int CT, int HD>
-__global__ void __launch_bounds__(128) paged_attn_simple_kernel(const AttnArgs a) {
-  constexpr bool BF = CT == CT_BF16;
-  constexpr int kPer = HD / 32;
-  __shared__ float qs[4][HD];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t unit = blockIdx.x * 4ll + warp;
-  const int t = static_cast<int>(unit / a.heads), h = static_cast<int>(unit % a.heads), g = h / a.group;
-  if (t >= a.n_tokens || t >= a.q_start[a.n_req]) return;
-  int lo = 0, hi = a.n_req - 1;   // the request of row t: the last one that starts at or before it
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.q_start[mid] <= t) lo = mid;
-    else hi = mid - 1;
-  }
-  const int b = lo, n = a.q_start[b + 1] - a.q_start[b];
-  if (min(n, a.max_new) * a.group <= a.rows_limit) return;
-  if (t - a.q_start[b] >= a.max_new) return;
-  const int total = static_cast<int>(min(static_cast<int64_t>(a.kv_len[b]), static_cast<int64_t>(a.width) << a.shift));
-  const int lim = min(total, a.kv_len[b] - n + (t - a.q_start[b]) + 1);   // keys < lim
-  for (int d = lane; d < HD; d += 32) qs[warp][d] = up16<BF>(a.q[t * a.q_tok + h * a.q_head + d]) * a.scale;
-  __syncwarp();
-  const int32_t* tab = a.table + b * a.table_ld;
-  float m = -INFINITY, l = 0.f, acc[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
-  auto value = [&](const void* base, const void* sbase, const int64_t* st, const int64_t* ss, int key, int d) -> float {
-    const int page = tab[key >> a.shift];
-    if (page < 0 || page >= a.c.pages) return 0.f;
-    const int in = key & (a.c.page_size - 1);
-    const int64_t at = page * st[0] + g * st[1] + in * st[2] + d;
-    if constexpr (CT == CT_Q8) {
-      const float s = __half2float(static_cast<const __half*>(sbase)[page * ss[0] + g * ss[1] + in * ss[2] + (d >> 5)]);
-      const float v = static_cast<float>(static_cast<int>(static_cast<const uint8_t*>(base)[at]) - 128) * s;
-      return __half2float(__float2half(v));
-    } else {
-      return up16<BF>(static_cast<const uint16_t*>(base)[at]);
+    for (int p = p0; p < p1; ++p) {
+      const float4 v =
+          *reinterpret_cast<const float4*>(a.part + (static_cast<int64_t>(slot_of(p)) * ROWS + row) * HD + 4 * lane);
+      const float w = wgt[p];
+      s.x = fmaf(v.x, w, s.x);
+      s.y = fmaf(v.y, w, s.y);
+      s.z = fmaf(v.z, w, s.z);
+      s.w = fmaf(v.w, w, s.w);
     }
-  };
-  for (int k0 = 0; k0 < lim; k0 += 32) {
-    const int key = k0 + lane;
-    float s = -INFINITY;
-    if (key < lim) {
-      s = 0.f;
-      for (int d = 0; d < HD; ++d) s = fmaf(qs[warp][d], value(a.c.k, a.c.k_scale, a.c.k_stride, a.c.ks_stride, key, d), s);
+    acc[tid] = s;
+    __syncthreads();
+    if (grp == 0) {
+      for (int k = 1; k < kGroups; ++k) {
+        const float4 v = acc[k * kLanes + lane];
+        s.x += v.x;
+        s.y += v.y;
+        s.z += v.z;
+        s.w += v.w;
+      }
+      const int t = t0 + row / a.group, hq = head * a.group + row % a.group;
+      const bool sees = min(r.keys, r.kv - r.n_all + t + 1) > 0;
+      float v[4] = {s.x / l, s.y / l, s.z / l, s.w / l};
+      const int64_t tok = r.q0 + t;
+      if (a.gate) {
+        const uint2 x = *reinterpret_cast<const uint2*>(a.gate + tok * a.g_tok + hq * a.g_head + 4 * lane);
+        const float2 x0 = unpack2<BF>(x.x), x1 = unpack2<BF>(x.y);
+        v[0] /= 1.f + __expf(-x0.x);
+        v[1] /= 1.f + __expf(-x0.y);
+        v[2] /= 1.f + __expf(-x1.x);
+        v[3] /= 1.f + __expf(-x1.y);
+      }
+      if (!sees) v[0] = v[1] = v[2] = v[3] = 0.f;
+      *reinterpret_cast<uint2*>(a.out + tok * a.o_tok + hq * a.o_head + 4 * lane) =
+          make_uint2(pack2<BF>(v[0], v[1]), pack2<BF>(v[2], v[3]));
     }
-    float mt = s;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
-    const float mn = fmaxf(m, mt);
-    const float base = mn == -INFINITY ? 0.f : mn;
-    const float cor = __expf(m - base), p = __expf(s - base);
-    m = mn;
-    l = l * cor + p;   // per lane; summed at the end
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) acc[i] *= cor;
-    for (int j = 0; j < min(32, lim - k0); ++j) {
-      const float pj = __shfl_sync(0xffffffffu, p, j);
-#pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        acc[i] = fmaf(pj, value(a.c.v, a.c.v_scale, a.c.v_stride, a.c.vs_stride, k0 + j, lane + 32 * i), acc[i]);
-    }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int d = lane + 32 * i;
-    float o = lim > 0 ? acc[i] / l : 0.f;
-    if (a.gate) o /= 1.f + __expf(-up16<BF>(a.gate[t * a.g_tok + h * a.g_head + d]));
-    a.out[t * a.o_tok + h * a.o_head + d] = down16<BF>(o);
   }
 }
 
@@ -872,21 +1527,35 @@ int launch_rows(AttnArgs a, void* ws, int sms, cudaStream_t s) {
   return launch_dependent(reinterpret_cast<const void*>(paged_combine_kernel<CT == CT_BF16, HD, kRowsMax>),
                           dim3(static_cast<unsigned>(std::min<int64_t>(items, ctas)), most), dim3(256), s, args);
 }
-template <int CT>
-int launch_rows_hd(const AttnArgs& a, void* ws, int sms, cudaStream_t s) {
-  if (a.c.head_dim == 256) return launch_rows<CT, 256>(a, ws, sms, s);
-  if (a.c.head_dim == 128) return launch_rows<CT, 128>(a, ws, sms, s);
-  return launch_rows<CT, 64>(a, ws, sms, s);
+template <int CT, int HD>
+int launch_tiles(AttnArgs a, void* ws, int sms, cudaStream_t s) {
+  using C = TilesCfg<CT, HD>;
+  static bool configured = false;
+  if (!configured) {
+    if (cudaFuncSetAttribute(paged_tiles_kernel<CT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) !=
+        cudaSuccess)
+      return TLX_ERR_LAUNCH;
+    configured = true;
+  }
+  const int ctas = sms * C::kCtas;
+  set_split(a, ws, split_area(ctas, 128, HD));
+  a.by_item = 0;
+  paged_tiles_kernel<CT, HD><<<ctas, C::kThreads, C::kSmem, s>>>(a, static_cast<uint32_t*>(ws));
+  if (cudaGetLastError() != cudaSuccess) return TLX_ERR_LAUNCH;
+  void* args[] = {&a};
+  return launch_dependent(reinterpret_cast<const void*>(paged_combine_kernel<CT == CT_BF16, HD, 128>),
+                          dim3(ctas, 16), dim3(256), s, args);
 }
-
 template <int CT>
-int launch_simple(const AttnArgs& a, cudaStream_t s) {
-  const int64_t units = static_cast<int64_t>(a.n_tokens) * a.heads;
-  const unsigned grid = static_cast<unsigned>((units + 3) / 4);
-  if (a.c.head_dim == 256) paged_attn_simple_kernel<CT, 256><<<grid, 128, 0, s>>>(a);
-  else if (a.c.head_dim == 128) paged_attn_simple_kernel<CT, 128><<<grid, 128, 0, s>>>(a);
-  else paged_attn_simple_kernel<CT, 64><<<grid, 128, 0, s>>>(a);
-  return cudaGetLastError() == cudaSuccess ? TLX_OK : TLX_ERR_LAUNCH;
+int launch_hd(const AttnArgs& a, bool tiles, void* ws, int sms, cudaStream_t s) {
+  if (a.c.head_dim == 256) return tiles ? launch_tiles<CT, 256>(a, ws, sms, s) : launch_rows<CT, 256>(a, ws, sms, s);
+  if (a.c.head_dim == 128) return tiles ? launch_tiles<CT, 128>(a, ws, sms, s) : launch_rows<CT, 128>(a, ws, sms, s);
+  return tiles ? launch_tiles<CT, 64>(a, ws, sms, s) : launch_rows<CT, 64>(a, ws, sms, s);
+}
+int launch_form(const AttnArgs& a, int ct, bool tiles, void* ws, int sms, cudaStream_t s) {
+  if (ct == CT_F16) return launch_hd<CT_F16>(a, tiles, ws, sms, s);
+  if (ct == CT_BF16) return launch_hd<CT_BF16>(a, tiles, ws, sms, s);
+  return launch_hd<CT_Q8>(a, tiles, ws, sms, s);
 }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -902,7 +1571,9 @@ size_t tlx_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim
   if (heads < 1 || kv_heads < 1 || kv_heads > 1024 || heads % kv_heads || heads / kv_heads > 128 ||
       (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return 0;
-  return split_area(sm_count() * kRowsCtasPerSm, kRowsMax, head_dim).end;
+  const int sms = sm_count();
+  return std::max(split_area(sms * kRowsCtasPerSm, kRowsMax, head_dim).end,
+                  split_area(sms * (head_dim == 256 ? 1 : 2), 128, head_dim).end);
 }
 
 int tlx_paged_attention(const tlx_paged_kv* cache, const int32_t* block_table, int64_t table_stride, int table_width,
@@ -951,18 +1622,14 @@ int tlx_paged_attention(const tlx_paged_kv* cache, const int32_t* block_table, i
   a.o_tok = out_tok_stride;
   a.o_head = out_head_stride;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int ct = cache_type(cache);
-  if (a.group <= kRowsMax) {   // the requests' lengths are on the device: the forms share them out there
-    const int sms = sm_count();
-    const int rr = ct == CT_F16    ? launch_rows_hd<CT_F16>(a, ws, sms, s)
-                   : ct == CT_BF16 ? launch_rows_hd<CT_BF16>(a, ws, sms, s)
-                                   : launch_rows_hd<CT_Q8>(a, ws, sms, s);
-    if (rr) return rr;
+  // the requests' lengths are on the device, so each form picks its own requests there
+  const int ct = cache_type(cache), sms = sm_count();
+  if (a.group <= kRowsMax) {
+    const int rows_rc = launch_form(a, ct, false, ws, sms, s);
+    if (rows_rc) return rows_rc;
   }
   if (static_cast<int64_t>(a.max_new) * a.group <= kRowsMax) return TLX_OK;
-  if (ct == CT_F16) return launch_simple<CT_F16>(a, s);
-  if (ct == CT_BF16) return launch_simple<CT_BF16>(a, s);
-  return launch_simple<CT_Q8>(a, s);
+  return launch_form(a, ct, true, ws, sms, s);
 }
 
 }  // extern "C"
