@@ -13,6 +13,8 @@
 //   tokens, a few drafts): bound by the cache's bytes, so a warp-level matrix product on
 //   16 rows is enough and the decoded keys never leave registers.
 // tiles form (paged_tiles_kernel)  the rest: tcgen05 on tiles of 128 query rows.
+#include <cuda.h>
+
 #include <algorithm>
 
 #include "paged.cuh"
@@ -185,6 +187,8 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;\n" ::: "memory"); }
+
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -226,6 +230,15 @@ template <bool BF>
 __device__ __forceinline__ bool bad16(uint32_t w) {
   constexpr uint32_t e = BF ? 0x7F80u : 0x7C00u;
   return (w & e) == e || (w & (e << 16)) == (e << 16);
+}
+
+// takes infinite and NaN halves out of w; whether there was one
+template <bool BF>
+__device__ __forceinline__ bool drop_bad(uint32_t& w) {
+  constexpr uint32_t e = BF ? 0x7F80u : 0x7C00u;
+  const bool lo = (w & e) == e, hi = (w & (e << 16)) == (e << 16);
+  w &= (lo ? 0xFFFF0000u : 0xFFFFFFFFu) & (hi ? 0x0000FFFFu : 0xFFFFFFFFu);
+  return lo || hi;
 }
 
 template <int CT, int HD>
@@ -637,9 +650,22 @@ __global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel
 //   warps 0..3   softmax, one thread per row; O is rescaled (in tensor memory) only when a
 //                row's maximum grows by more than 2^8, which keeps P in range
 //   warp 4       one thread issues the MMAs, S(i + 1) ahead of O += P(i) V(i)
-//   warps 5..    K and V halves of the units into a ring, in the order the MMAs read them
+//   warp 5       loads the K and V halves of the units, in the order the MMAs read them:
+//                one TMA box per page (and 64 dims), so pages may lie anywhere and what is
+//                outside the pool reads as 0
+//   warps 6..    16-bit caches: on the MMA thread's request take out of V what must not
+//                reach the product (rows past the last key, and infinite or NaN values where
+//                some rows do not see the unit whole); int8 caches: turn every half into
+//                fp16(code * scale)
 // Every wait is bounded: a timeout raises the error word, all roles leave, issued MMAs
 // and copies are drained and tensor memory is freed.
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* b) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(b))
+      : "memory");
+}
 __device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t parity) {
   const bool ok = tc_wait(b, parity);
   __syncwarp();   // what follows is for the whole warp
@@ -654,14 +680,19 @@ struct TilesCfg {
   static constexpr bool kQTmem = HD == 256;
   static constexpr int kQBytes = kQTmem ? 0 : 128 * HD * 2;
   static constexpr int kPBytes = 128 * kKeys * 2;
-  static constexpr int kPBufs = HD == 128 ? 1 : 2;
-  static constexpr int kRing = HD == 64 ? 6 : HD == 128 ? 4 : 6;
-  static constexpr int kProducers = HD == 256 ? 7 : 3;          // warps
-  static constexpr int kThreads = 32 * (5 + kProducers);
+  static constexpr int kPBufs = HD == 128 || (kQ8 && HD == 256) ? 1 : 2;
+  // 16-bit halves of K or V that the MMAs read, and (int8) halves as they lie in the cache
+  static constexpr int kRing = kQ8 ? (HD == 128 ? 2 : 4) : HD == 128 ? 4 : 6;
+  static constexpr int kRaw = !kQ8 ? 0 : HD == 128 ? 3 : 4;
+  static constexpr int kRawHalf = kKeys * HD;                   // codes; the scales follow
+  static constexpr int kRawBytes = kRawHalf + kKeys * (HD / 16);
+  static constexpr int kThreads = HD == 256 ? 384 : 256;
+  static constexpr int kHelpers = kThreads / 32 - 6;            // warps
   static constexpr int kCtas = HD == 256 ? 1 : 2;               // on an SM
   static constexpr int kOffP = kRing * kHalf;
   static constexpr int kOffQ = kOffP + kPBufs * kPBytes;
-  static constexpr int kOffBar = kOffQ + kQBytes;
+  static constexpr int kOffRaw = kOffQ + kQBytes;
+  static constexpr int kOffBar = kOffRaw + kRaw * kRawBytes;
   static constexpr int kSmem = kOffBar + 512;
   static constexpr uint32_t kTmem = HD == 256 ? 512 : 256;
   static constexpr uint32_t kColS = 0, kColO = 128;
@@ -722,7 +753,7 @@ __device__ __forceinline__ int64_t units_before(const AttnArgs& a, const Req& r,
   return s;
 }
 
-// The producers replace infinite and NaN values of V by 0 in the units that some rows do
+// The helpers replace infinite and NaN values of V by 0 in the units that some rows do
 // not see whole (0 * inf in the product would reach those rows); this adds weight * value
 // of such keys to the rows that do see them.  Called by whole warps with O at rest; the
 // weights are the rounded ones of the product, from P in shared memory.
@@ -762,33 +793,42 @@ __device__ __noinline__ void restore_bad_values(const AttnArgs& a, int b, int he
 
 template <int CT, int HD>
 __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::kCtas)
-    paged_tiles_kernel(const __grid_constant__ AttnArgs a, uint32_t* err) {
+    paged_tiles_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap k_map,
+                       const __grid_constant__ CUtensorMap v_map, uint32_t* err) {
   using C = TilesCfg<CT, HD>;
   constexpr bool BF = CT == CT_BF16, Q8 = C::kQ8;
   static_assert(C::kColO + HD + (C::kQTmem ? C::kColQ - 384 + HD / 2 : 0) <= C::kTmem, "tensor memory");
-  constexpr int NP = C::kProducers, RING = C::kRing, PB = C::kPBufs;
+  constexpr int NH = C::kHelpers, RING = C::kRing, PB = C::kPBufs;
   extern __shared__ __align__(1024) uint8_t sm_tiles[];
   uint8_t* const sm = sm_tiles;
   uint64_t* bar = reinterpret_cast<uint64_t*>(sm + C::kOffBar);
-  uint64_t* full = bar;                 // [RING] producers -> MMA
-  uint64_t* empty = full + RING;        // [RING] MMA -> producers
-  uint64_t* s_full = empty + RING;      // [2] MMA -> softmax
+  uint64_t* landed = bar;               // [8] TMA -> MMA or helpers
+  uint64_t* raw_free = landed + 8;      // [RAW] helpers -> loader
+  uint64_t* full = raw_free + 8;        // [RING] helpers -> MMA
+  uint64_t* empty = full + 8;           // [RING] MMA -> loader or helpers
+  uint64_t* s_full = empty + 8;         // [2] MMA -> softmax
   uint64_t* s_free = s_full + 2;        // [2] softmax -> MMA
   uint64_t* p_full = s_free + 2;        // [2] softmax -> MMA
   uint64_t* pv_done = p_full + 2;       // [2] MMA -> softmax
   uint64_t* q_full = pv_done + 2;       // softmax -> MMA: Q of the next item is in
   uint64_t* o_free = q_full + 1;        // softmax -> MMA: O of the last item is read
-  uint64_t* done = o_free + 1;
+  uint64_t* fix_req = o_free + 1;       // MMA -> helpers: a V half to clean
+  uint64_t* fix_done = fix_req + 1;     // helpers -> MMA
+  uint64_t* done = fix_done + 1;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(done + 1);
   volatile uint32_t* abort_flag = tmem_holder + 1;
-  // [8] by unit: unit + 1 if the producers took a bad value out of its V (they are fewer
-  // than 8 units ahead of the softmax)
+  // [8] by unit: unit + 1 if the helpers took a bad value out of its V (they are fewer than
+  // 8 units ahead of the softmax)
   volatile int* bad = reinterpret_cast<int*>(tmem_holder + 2);
   struct First {
     int tile, head, u;
   };
   First* first_at = reinterpret_cast<First*>(tmem_holder + 10);
-  static_assert((2 * RING + 11) * 8 + 10 * 4 + sizeof(First) <= 512, "barrier area");
+  struct Fix {
+    int slot, valid, edge, unit;   // ring slot (-1: no more), keys of the unit that exist
+  };
+  Fix* fix = reinterpret_cast<Fix*>(tmem_holder + 14);
+  static_assert((4 * 8 + 13) * 8 + 14 * 4 + sizeof(Fix) <= 512 && RING <= 8 && C::kRaw <= 8, "barrier area");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   griddep_launch_dependents();
@@ -823,8 +863,10 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
     }
   }
   if (tid == 0) {
-    for (int i = 0; i < RING; ++i) {
-      mbar_init(&full[i], NP);
+    for (int i = 0; i < 8; ++i) {
+      mbar_init(&landed[i], Q8 ? 33 : 1);   // int8: 32 lanes' copies of the scales as well
+      mbar_init(&raw_free[i], NH);
+      mbar_init(&full[i], NH);
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 8; ++i) bad[i] = 0;
@@ -836,6 +878,8 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
     }
     mbar_init(q_full, 4);
     mbar_init(o_free, 4);
+    mbar_init(fix_req, 1);
+    mbar_init(fix_done, NH);
     mbar_init(done, 1);
     *abort_flag = 0u;
     mbar_fence_init();
@@ -879,15 +923,23 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
     }
   };
 
+  // V of a unit that some row of the tile does not see whole, and the keys it really has
+  auto is_edge = [&](const Pos& p) {
+    return max(0, min(p.r.keys, p.r.kv - p.r.n_all + p.tile * tile_tokens(a) + 1)) < min(p.u * 64 + 64, p.r.keys);
+  };
+  auto is_special = [&](const Pos& p) { return p.u * 64 + 64 > p.r.keys || is_edge(p); };
+
   if (warp == 4) {
     // --------------------------------------------------------------- MMA issuer
     if (lane == 0) {
-      int h = 0;          // ring halves consumed
+      int h = 0;               // ring halves consumed
+      int fixes = 0;           // 16-bit: V halves the helpers were asked to clean
       int item = 0, left = min(at.of - at.u, n);   // units left of the current item
       auto issue_qk = [&](int i, bool starts, int it) -> bool {
         const int b = i & 1, slot = h % RING;
         if (starts && !tc_wait(q_full, it & 1)) return false;
-        if (!tc_wait(&full[slot], (h / RING) & 1) || !tc_wait(&s_free[b], ((i >> 1) & 1) ^ 1)) return false;
+        if (!tc_wait(Q8 ? &full[slot] : &landed[slot], (h / RING) & 1) || !tc_wait(&s_free[b], ((i >> 1) & 1) ^ 1))
+          return false;
         tc_after();
         const uint32_t kb = sbase + slot * C::kHalf;
 #pragma unroll
@@ -907,7 +959,13 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
       auto issue_pv = [&](int i, bool starts, int it) -> bool {
         const int slot = h % RING, pb = PB == 2 ? i & 1 : 0;
         if (starts && it > 0 && !tc_wait(o_free, (it - 1) & 1)) return false;
-        if (!tc_wait(&full[slot], (h / RING) & 1) || !tc_wait(&p_full[i & 1], (i >> 1) & 1)) return false;
+        if (!tc_wait(Q8 ? &full[slot] : &landed[slot], (h / RING) & 1)) return false;
+        if (!Q8 && is_special(at)) {
+          *fix = Fix{slot, at.r.keys - at.u * 64, is_edge(at), i};
+          mbar_arrive(fix_req);
+          if (!tc_wait(fix_done, fixes++ & 1)) return false;
+        }
+        if (!tc_wait(&p_full[i & 1], (i >> 1) & 1)) return false;
         tc_after();
         const uint32_t vb = sbase + slot * C::kHalf;
 #pragma unroll
@@ -924,6 +982,7 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
         const bool ends = --left == 0;
         if (!ends && i + 1 < n) ok = issue_qk(i + 1, false, item);
         ok = ok && issue_pv(i, starts, item);
+        ++at.u;
         starts = ends;
         if (ends && i + 1 < n) {
           next_item(at);
@@ -933,6 +992,10 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
         }
       }
       if (!ok) fail();
+      if constexpr (!Q8) {
+        fix->slot = -1;
+        mbar_arrive(fix_req);
+      }
       tc_commit(done);   // every issued MMA has completed before tensor memory is released
       if (!tc_wait(done, 0)) fail();
     }
@@ -1135,230 +1198,162 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
       at = next;
     }
     if (!ok) fail();
-  } else {
-    // --------------------------------------------------------------- producers
-    // The halves in MMA order: K(0), then per unit K(i + 1) and V(i), with V(i) first
-    // where unit i ends an item.  A warp moves every NP-th group of 32 16-byte chunks.
-    const int pw = warp - 5;
-    constexpr int CPK = HD * (Q8 ? 1 : 2) / 16;          // 16-byte chunks of a cached row
-    constexpr int OPS = 64 * CPK / 32;                   // warp operations of a half
-    constexpr int PER = (OPS + NP - 1) / NP;
-    bool ok = true;
+  } else if (warp == 5) {
+    // ------------------------------------------------------------------ loader
+    // Halves in MMA order: per unit K(i) then V(i - 1), or V(i - 1) first where unit i
+    // starts an item.  A lane owns one TMA box of a half: 64 dims (int8: all) of the keys
+    // of one page.
+    constexpr int ATOMS = Q8 ? 1 : HD / 64, LR = Q8 ? C::kRaw : RING;
+    const int rows = min(a.c.page_size, 64), part = lane / ATOMS, atom = lane % ATOMS;
+    const bool mine = part * rows < 64;
+    auto page_of = [&](const Pos& p) -> int {   // -1: outside the pool, read as 0
+      const int key = p.u * 64 + part * rows;
+      return mine && key < p.r.keys ? a.table[p.b * a.table_ld + (key >> a.shift)] : -1;
+    };
     int h = 0;
-    Pos kp = at, vp = at;    // units of the next K and V halves
-    int ki = 0, vi = 0, kleft = min(at.of - at.u, n), vleft = kleft;
-    auto step = [&](Pos& p, int& idx, int& left) {   // to the next unit
-      ++idx;
-      ++p.u;
-      if (--left == 0 && idx < n) {
-        next_item(p);
-        left = p.of;
-      }
-    };
-    // rows of the half's 64 keys: lane l holds keys l and l + 32
-    struct Rows {
-      int64_t off[2], soff[2];
-      uint32_t ok[2];
-    };
-    auto find_rows = [&](const Pos& p, bool v, Rows& w) {
-      const int64_t* cs = v ? a.c.v_stride : a.c.k_stride;
-      const int64_t* ss = v ? a.c.vs_stride : a.c.ks_stride;
+    bool ok = true;
+    auto load = [&](bool v, int page, int u, int head, int keys) {
+      const int slot = h % LR;
+      if (!(ok = warp_wait(Q8 ? &raw_free[slot] : &empty[slot], ((h / LR) & 1) ^ 1))) return;
+      if (lane == 0) mbar_arrive_expect_tx(&landed[slot], Q8 ? C::kRawHalf : C::kHalf);
+      __syncwarp();
+      const int in = (u * 64 + part * rows) & (a.c.page_size - 1);
+      uint8_t* dst = Q8 ? sm + C::kOffRaw + slot * C::kRawBytes + part * rows * HD
+                        : sm + slot * C::kHalf + atom * 8192 + part * rows * 128;
+      if (mine) tma_load_4d(dst, v ? &v_map : &k_map, atom * 64, in, head, page, &landed[slot]);
+      if constexpr (Q8) {
+        const uint16_t* sc = static_cast<const uint16_t*>(v ? a.c.v_scale : a.c.k_scale);
+        const int64_t* ss = v ? a.c.vs_stride : a.c.ks_stride;
+        const uint32_t sb = sbase + C::kOffRaw + slot * C::kRawBytes + C::kRawHalf;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int key = p.u * 64 + x * 32 + lane;
-        w.off[x] = 0;
-        w.soff[x] = 0;
-        bool in_pool = key < p.r.keys;
-        if (in_pool) {
-          const int page = a.table[p.b * a.table_ld + (key >> a.shift)];
-          in_pool = page >= 0 && page < a.c.pages;
-          if (in_pool) {
-            const int64_t in = key & (a.c.page_size - 1);
-            w.off[x] = (page * cs[0] + p.head * cs[1] + in * cs[2]) * (Q8 ? 1 : 2);
-            if constexpr (Q8) w.soff[x] = page * ss[0] + p.head * ss[1] + in * ss[2];
-          }
+        for (int x = 0; x < 2; ++x) {
+          const int k = x * 32 + lane, key = u * 64 + k;
+          const int pg = __shfl_sync(0xffffffffu, page, k / rows);
+          const bool in_pool = key < keys && pg >= 0 && pg < a.c.pages;
+          const uint16_t* src = in_pool ? sc + pg * ss[0] + head * ss[1] + (key & (a.c.page_size - 1)) * ss[2] : sc;
+          cp_async_small<HD / 16>(sb + k * (HD / 16), src, in_pool);
         }
-        w.ok[x] = __ballot_sync(0xffffffffu, in_pool);
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(smem_u32(&landed[slot])) : "memory");
       }
+      ++h;
     };
-    // V of a unit that some row of the tile does not see whole: bad values are taken out
-    auto is_edge = [&](const Pos& p) {
-      return max(0, min(p.r.keys, p.r.kv - p.r.n_all + p.tile * tile_tokens(a) + 1)) < min(p.u * 64 + 64, p.r.keys);
-    };
-    const int total = 2 * n;
-    bool k_turn = true;
-    auto after = [&](bool v) {   // order of the halves
-      if (!v) {
-        step(kp, ki, kleft);
-        k_turn = ki == 1 + vi ? (ki < n && vleft != 1) : false;
-      } else {
-        step(vp, vi, vleft);
-        k_turn = ki < n && (ki == vi || vleft != 1);
+    int pk = page_of(at), pv = -1, u_v = 0, head_v = 0, keys_v = 0, left = min(at.of - at.u, n);
+    bool starts = true;
+    for (int i = 0; i <= n && ok && !*abort_flag; ++i) {
+      if (i > 0 && (starts || i == n)) load(true, pv, u_v, head_v, keys_v);
+      if (i == n || !ok) break;
+      load(false, pk, at.u, at.head, at.r.keys);
+      if (i > 0 && !starts && ok) load(true, pv, u_v, head_v, keys_v);
+      pv = pk;
+      u_v = at.u;
+      head_v = at.head;
+      keys_v = at.r.keys;
+      starts = --left == 0;
+      if (i + 1 < n) {
+        if (starts) {
+          next_item(at);
+          left = at.of;
+        } else {
+          ++at.u;
+        }
+        pk = page_of(at);   // in flight while the ring is full
       }
-    };
+    }
+    if (!ok) fail();
+    if (!ok || *abort_flag) {   // no copy may still be in flight when the CTA ends
+      if constexpr (Q8) cp_async_wait_all();
+      for (int f = max(0, h - LR); f < h; ++f) tc_wait(&landed[f % LR], (f / LR) & 1);
+    }
+  } else {
+    // ----------------------------------------------------------------- helpers
+    const int hw = warp - 6;
+    bool ok = true;
     if constexpr (!Q8) {
-      constexpr int AHEAD = RING - 2;
-      uint32_t edge_of = 0;             // bit (half % 32): that half needs the check
-      int unit_of[RING];
-      auto finish = [&](int f) {        // half f has landed
-        const int slot = f % RING;
-        if ((edge_of >> (f & 31)) & 1) {
-          uint8_t* hb = sm + slot * C::kHalf;
-          bool any_bad = false;
-          for (int x = 0; x < PER; ++x) {
-            const int op = pw + NP * x;
-            if (op >= OPS) break;
-            const int idx = op * 32 + lane, key = idx / CPK, ch = idx % CPK;
-            uint4* p = reinterpret_cast<uint4*>(hb + (ch >> 3) * 8192 + sw128(key, ch & 7));
-            uint4 v = *p;
-            uint32_t w[4] = {v.x, v.y, v.z, v.w};
-            bool mine = false;
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              if (bad16<BF>(w[y] & 0xFFFFu)) {
-                w[y] &= 0xFFFF0000u;
-                mine = true;
-              }
-              if (bad16<BF>(w[y] >> 16)) {
-                w[y] &= 0xFFFFu;
-                mine = true;
-              }
-            }
-            if (mine) {
+      for (int k = 0; ok && !*abort_flag; ++k) {
+        if (!(ok = warp_wait(fix_req, k & 1))) break;
+        const Fix f = *fix;
+        if (f.slot < 0) break;
+        uint8_t* hb = sm + f.slot * C::kHalf;
+        bool any_bad = false;
+        for (int idx = hw * 32 + lane; idx < 64 * HD / 8; idx += NH * 32) {
+          const int key = idx / (HD / 8), ch = idx % (HD / 8);
+          uint4* p = reinterpret_cast<uint4*>(hb + (ch >> 3) * 8192 + sw128(key, ch & 7));
+          if (key >= f.valid) {
+            *p = make_uint4(0u, 0u, 0u, 0u);
+          } else if (f.edge) {
+            const uint4 x = *p;
+            uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            if (drop_bad<BF>(w[0]) | drop_bad<BF>(w[1]) | drop_bad<BF>(w[2]) | drop_bad<BF>(w[3])) {
               *p = make_uint4(w[0], w[1], w[2], w[3]);
               any_bad = true;
             }
           }
-          if (any_bad) {
-            int u = 0;
-#pragma unroll
-            for (int x = 0; x < RING; ++x)
-              if (x == slot) u = unit_of[x];
-            bad[u & 7] = u + 1;
-          }
         }
+        if (any_bad) bad[f.unit & 7] = f.unit + 1;
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&full[slot]);
-      };
-      for (; h < total && ok && !*abort_flag; ++h) {
-        const int slot = h % RING;
-        const bool v = !k_turn;
-        Rows w;
-        edge_of &= ~(1u << (h & 31));
-        if (v) {
-          find_rows(vp, true, w);
-          if (is_edge(vp)) edge_of |= 1u << (h & 31);
-        } else {
-          find_rows(kp, false, w);
-        }
-#pragma unroll
-        for (int x = 0; x < RING; ++x)
-          if (x == slot) unit_of[x] = v ? vi : ki;
-        if (!(ok = tc_wait(&empty[slot], ((h / RING) & 1) ^ 1))) break;
-        const uint8_t* base = static_cast<const uint8_t*>(v ? a.c.v : a.c.k);
-        const uint32_t hb = sbase + slot * C::kHalf;
-#pragma unroll 8
-        for (int x = 0; x < PER; ++x) {
-          const int op = pw + NP * x;
-          if (op < OPS) {
-            const int idx = op * 32 + lane, key = idx / CPK, ch = idx % CPK;
-            const bool hi = op * 32 / CPK >= 32;   // the same for the warp
-            const int64_t off = __shfl_sync(0xffffffffu, hi ? w.off[1] : w.off[0], key & 31);
-            const bool in_pool = ((hi ? w.ok[1] : w.ok[0]) >> (key & 31)) & 1;
-            cp_async16(hb + (ch >> 3) * 8192 + sw128(key, ch & 7), base + off + ch * 16, in_pool);
-          }
-        }
-        cp_async_commit();
-        after(v);
-        if (h >= AHEAD) {
-          cp_async_wait<AHEAD>();
-          finish(h - AHEAD);
-        }
+        if (lane == 0) mbar_arrive(fix_done);
       }
-      cp_async_wait<0>();
-      if (ok && !*abort_flag)
-        for (int f = max(0, total - AHEAD); f < total; ++f) finish(f);
     } else {
-      // codes into registers one half ahead, then fp16(code * scale) into the ring
-      uint4 cur[PER], nxt[PER];
-      uint16_t cs[PER], ns[PER];
-      auto fetch = [&](bool v, uint4 (&q)[PER], uint16_t (&sc)[PER]) {
-        Rows w;
-        if (v) find_rows(vp, true, w);
-        else find_rows(kp, false, w);
-        const uint8_t* base = static_cast<const uint8_t*>(v ? a.c.v : a.c.k);
-        const uint16_t* sb = static_cast<const uint16_t*>(v ? a.c.v_scale : a.c.k_scale);
-#pragma unroll
-        for (int x = 0; x < PER; ++x) {
-          const int op = pw + NP * x;
-          q[x] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-          sc[x] = 0;
-          if (op < OPS) {
-            const int idx = op * 32 + lane, key = idx / CPK, ch = idx % CPK;
-            const bool hi = op * 32 / CPK >= 32;
-            const int64_t off = __shfl_sync(0xffffffffu, hi ? w.off[1] : w.off[0], key & 31);
-            const int64_t so = __shfl_sync(0xffffffffu, hi ? w.soff[1] : w.soff[0], key & 31);
-            if (((hi ? w.ok[1] : w.ok[0]) >> (key & 31)) & 1) {
-              q[x] = __ldg(reinterpret_cast<const uint4*>(base + off + ch * 16));
-              sc[x] = __ldg(sb + so + (ch >> 1));
-            }
-          }
-        }
-      };
-      bool v = !k_turn;
-      fetch(v, nxt, ns);
-      for (; h < total && ok && !*abort_flag; ++h) {
-        const int slot = h % RING;
-        const bool edge = v && is_edge(vp);
-        const int unit = v ? vi : ki;
-#pragma unroll
-        for (int x = 0; x < PER; ++x) {
-          cur[x] = nxt[x];
-          cs[x] = ns[x];
-        }
-        after(v);
-        if (h + 1 < total) {
-          v = !k_turn;
-          fetch(v, nxt, ns);   // in flight while this half is written
-        }
-        if (!(ok = tc_wait(&empty[slot], ((h / RING) & 1) ^ 1))) break;
+      constexpr int CPK = HD / 16;   // 16-byte chunks of a cached row
+      int h = 0;
+      auto convert = [&](bool v, int valid, bool edge, int unit) {
+        const int slot = h % RING, rs = h % C::kRaw;
+        if (!(ok = warp_wait(&landed[rs], (h / C::kRaw) & 1)) || !(ok = warp_wait(&empty[slot], ((h / RING) & 1) ^ 1))) return;
+        const uint8_t* raw = sm + C::kOffRaw + rs * C::kRawBytes;
         bool any_bad = false;
+#pragma unroll 4
+        for (int idx = hw * 32 + lane; idx < 64 * CPK; idx += NH * 32) {
+          const int key = idx / CPK, ch = idx % CPK;   // 16 dims: 16-bit chunks 2 ch and 2 ch + 1
+          const uint4 x = lds128(raw + idx * 16);
+          uint32_t sc = *reinterpret_cast<const uint16_t*>(raw + C::kRawHalf + key * (HD / 16) + (ch >> 1) * 2);
+          if (key >= valid) sc = 0u;   // rows past the last key: +-0
+          const uint32_t s2 = sc | sc << 16;
+          const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+          uint32_t o[8];
 #pragma unroll
-        for (int x = 0; x < PER; ++x) {
-          const int op = pw + NP * x;
-          if (op < OPS) {
-            const int idx = op * 32 + lane, key = idx / CPK, ch = idx % CPK;   // 16 dims: chunks 2 ch, 2 ch + 1
-            const uint32_t s2 = cs[x] | static_cast<uint32_t>(cs[x]) << 16;
-            const uint32_t in[4] = {cur[x].x, cur[x].y, cur[x].z, cur[x].w};
-            uint32_t o[8];
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              o[2 * y] = dq2(in[y], 0x5140u, s2);
-              o[2 * y + 1] = dq2(in[y], 0x7362u, s2);
-            }
-            if (edge) {
-#pragma unroll
-              for (int y = 0; y < 8; ++y) {
-                if (bad16<false>(o[y] & 0xFFFFu)) {
-                  o[y] &= 0xFFFF0000u;
-                  any_bad = true;
-                }
-                if (bad16<false>(o[y] >> 16)) {
-                  o[y] &= 0xFFFFu;
-                  any_bad = true;
-                }
-              }
-            }
-            uint8_t* hb = sm + slot * C::kHalf + (ch >> 2) * 8192;
-            *reinterpret_cast<uint4*>(hb + sw128(key, (2 * ch) & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
-            *reinterpret_cast<uint4*>(hb + sw128(key, (2 * ch + 1) & 7)) = make_uint4(o[4], o[5], o[6], o[7]);
+          for (int y = 0; y < 4; ++y) {
+            o[2 * y] = dq2(in[y], 0x5140u, s2);
+            o[2 * y + 1] = dq2(in[y], 0x7362u, s2);
           }
+          if (edge) {
+#pragma unroll
+            for (int y = 0; y < 8; ++y) any_bad |= drop_bad<false>(o[y]);
+          }
+          // lanes of neighbouring atoms write their two chunks in opposite order: all banks once
+          const int first = (ch >> 2) & 1;
+          uint8_t* hb = sm + slot * C::kHalf + (ch >> 2) * 8192;
+          const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
+          *reinterpret_cast<uint4*>(hb + sw128(key, ((2 * ch) & 7) + first)) = first ? hi : lo;
+          *reinterpret_cast<uint4*>(hb + sw128(key, ((2 * ch) & 7) + (first ^ 1))) = first ? lo : hi;
         }
         if (any_bad) bad[unit & 7] = unit + 1;
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&full[slot]);
+        if (lane == 0) {
+          mbar_arrive(&full[slot]);
+          mbar_arrive(&raw_free[rs]);
+        }
+        ++h;
+      };
+      bool starts = true, edge_v = false;
+      int valid_v = 0, left = min(at.of - at.u, n);
+      for (int i = 0; i <= n && ok && !*abort_flag; ++i) {
+        if (i > 0 && (starts || i == n)) convert(true, valid_v, edge_v, i - 1);
+        if (i == n || !ok) break;
+        convert(false, at.r.keys - at.u * 64, false, i);
+        if (i > 0 && !starts && ok) convert(true, valid_v, edge_v, i - 1);
+        valid_v = at.r.keys - at.u * 64;
+        edge_v = is_edge(at);
+        starts = --left == 0;
+        if (i + 1 < n) {
+          if (starts) {
+            next_item(at);
+            left = at.of;
+          } else {
+            ++at.u;
+          }
+        }
       }
     }
     if (!ok) fail();
@@ -1527,6 +1522,37 @@ int launch_rows(AttnArgs a, void* ws, int sms, cudaStream_t s) {
   return launch_dependent(reinterpret_cast<const void*>(paged_combine_kernel<CT == CT_BF16, HD, kRowsMax>),
                           dim3(static_cast<unsigned>(std::min<int64_t>(items, ctas)), most), dim3(256), s, args);
 }
+// The pool as TMA sees it: [page][head][slot][dim], a box of 64 dims (int8: the row) of the
+// keys of one page that fall in a unit of 64.  A dimension of one entry takes any stride.
+bool page_map(CUtensorMap* map, const tlx_paged_kv& c, const void* base, const int64_t* stride) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static Encode enc = nullptr;   // looked up through the runtime: the library does not link the driver's
+  if (!enc) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return false;
+    enc = reinterpret_cast<Encode>(fn);
+  }
+  const bool q8 = c.dtype == TLX_DT_Q8;
+  const cuuint64_t esz = q8 ? 1 : 2;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.head_dim), static_cast<cuuint64_t>(c.page_size),
+                              static_cast<cuuint64_t>(c.kv_heads), static_cast<cuuint64_t>(c.pages)};
+  cuuint64_t strides[3];
+  for (int i = 0; i < 3; ++i)
+    strides[i] = dims[i + 1] > 1 ? static_cast<cuuint64_t>(stride[2 - i]) * esz : static_cast<cuuint64_t>(c.head_dim) * esz;
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(q8 ? c.head_dim : 64), static_cast<cuuint32_t>(std::min(c.page_size, 64)),
+                             1u, 1u};
+  const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+  return enc(map, q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims,
+             strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             q8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int CT, int HD>
 int launch_tiles(AttnArgs a, void* ws, int sms, cudaStream_t s) {
   using C = TilesCfg<CT, HD>;
@@ -1540,7 +1566,9 @@ int launch_tiles(AttnArgs a, void* ws, int sms, cudaStream_t s) {
   const int ctas = sms * C::kCtas;
   set_split(a, ws, split_area(ctas, 128, HD));
   a.by_item = 0;
-  paged_tiles_kernel<CT, HD><<<ctas, C::kThreads, C::kSmem, s>>>(a, static_cast<uint32_t*>(ws));
+  CUtensorMap km, vm;
+  if (!page_map(&km, a.c, a.c.k, a.c.k_stride) || !page_map(&vm, a.c, a.c.v, a.c.v_stride)) return TLX_ERR_LAUNCH;
+  paged_tiles_kernel<CT, HD><<<ctas, C::kThreads, C::kSmem, s>>>(a, km, vm, static_cast<uint32_t*>(ws));
   if (cudaGetLastError() != cudaSuccess) return TLX_ERR_LAUNCH;
   void* args[] = {&a};
   return launch_dependent(reinterpret_cast<const void*>(paged_combine_kernel<CT == CT_BF16, HD, 128>),
