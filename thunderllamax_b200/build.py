@@ -18,7 +18,7 @@ OUT = os.path.join(HERE, "libtlx_b200.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
 SOURCES = ["gemv.cu", "capi.cu", "moe.cu", "prefill.cu", "noalloc.cu", "lookup.cu", "attention.cu", "peer.cu", "w4a8.cu",
-           "paged.cu", "paged_attention.cu", "norm.cu"]
+           "paged.cu", "paged_attention.cu", "paged_rows.cu", "paged_tiles.cu", "norm.cu"]
 
 
 def nvcc() -> str:

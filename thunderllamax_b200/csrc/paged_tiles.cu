@@ -1,0 +1,890 @@
+// Tiles form of the paged attention: requests with more than 16 query rows per KV head.
+#include <cuda.h>
+
+#include "paged_attention.cuh"
+
+namespace tlx {
+namespace {
+
+// ----------------------------------------------------------------- tiles form
+// The 128 rows of a tensor-core tile are the query heads of one KV head times as many
+// tokens as fit (row = token * group + head), so every key read serves the whole group.
+// A CTA walks its units (64 keys of one item) on tcgen05:
+//   S(i) = Q K_i^T   M = 128, N = 64, K = head_dim; Q in tensor memory (head_dim 256) or
+//                    shared memory, S double-buffered in tensor memory
+//   O += P(i) V_i    M = 128, N = head_dim, K = 64; V is the MN-major operand as it lies
+//                    in the cache, P (16 bit) in shared memory, double-buffered where it fits
+//   softmax warpgroups   one thread per row; with two groups they take the units in turn,
+//                so one group's exponentials run beside the other's loads and waits, and
+//                hand on the row's reference maximum.  O is rescaled (in tensor memory) only
+//                when a row's maximum grows by more than 2^8, which keeps P in range.
+//   QK warp, PV warp     one thread each issues its MMAs: two issuers, because the waits and
+//                commits of one would leave the tensor pipe idle
+//   loader warp          the K and V halves of the units: one TMA box per page (and 64 dims),
+//                so pages may lie anywhere and what is outside the pool reads as 0
+//   helper warps         16-bit caches: on the PV thread's request take out of V what must
+//                not reach the product (rows past the last key, and infinite or NaN values
+//                where some rows do not see the unit whole); int8 caches: turn every half
+//                into fp16(code * scale)
+// Every wait is bounded: a timeout raises the error word, all roles leave, issued MMAs
+// and copies are drained and tensor memory is freed.
+template <int N>
+__device__ __forceinline__ void reg_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void reg_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N));
+}
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* b) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(b))
+      : "memory");
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t parity) {
+  const bool ok = tc_wait(b, parity);
+  __syncwarp();   // what follows is for the whole warp
+  return ok;
+}
+
+template <int CT, int HD>
+struct TilesCfg {
+  static constexpr bool kQ8 = CT == CT_Q8;
+  static constexpr int kKeys = 64;
+  static constexpr int kHalf = kKeys * HD * 2;                  // bytes of a K or V half
+  static constexpr bool kQTmem = HD == 256;
+  static constexpr int kQBytes = kQTmem ? 0 : 128 * HD * 2;
+  static constexpr int kPBytes = 128 * kKeys * 2;
+  // One CTA of two softmax groups on an SM, or (16-bit caches of narrow heads, whose smaller
+  // rings leave room) two CTAs of one group.
+  static constexpr int kGroups = HD == 256 || kQ8 ? 2 : 1;
+  static constexpr int kCtas = kGroups == 2 ? 1 : 2;
+  static constexpr int kPBufs = HD == 128 && !kQ8 ? 1 : 2;
+  // 16-bit halves of K or V that the MMAs read, and (int8) halves as they lie in the cache
+  static constexpr int kRing = kQ8 && HD == 256 ? 4 : HD == 128 && !kQ8 ? 4 : 6;
+  static constexpr int kRaw = !kQ8 ? 0 : HD == 256 ? 3 : 6;
+  static constexpr int kRawHalf = kKeys * HD;                   // codes; the scales follow
+  static constexpr int kRawBytes = kRawHalf + kKeys * (HD / 16);
+  static constexpr int kThreads = kGroups == 2 ? 512 : 256;
+  static constexpr int kQkWarp = 4 * kGroups, kPvWarp = kQkWarp + 1, kLoadWarp = kQkWarp + 2, kHelpWarp = kQkWarp + 3;
+  // int8: the four warps of the last warpgroup, a fixed share of the chunks each
+  static constexpr int kHelpFirst = kQ8 ? kThreads / 32 - 4 : kHelpWarp;
+  static constexpr int kHelpers = kThreads / 32 - kHelpFirst;
+  // registers after the roles part (of the 128 of the launch)
+  static constexpr int kRegsSoftmax = kGroups == 2 ? 168 : 184;
+  static constexpr int kRegsOther = kGroups == 2 ? 88 : 72;
+  static_assert(kGroups * kRegsSoftmax + (kThreads / 128 - kGroups) * kRegsOther <= kThreads, "register split");
+  static constexpr int kOffP = kRing * kHalf;
+  static constexpr int kOffQ = kOffP + kPBufs * kPBytes;
+  static constexpr int kOffRaw = kOffQ + kQBytes;
+  static constexpr int kOffX = kOffRaw + kRaw * kRawBytes;      // row maxima and sums the groups exchange
+  static constexpr int kOffBar = kOffX + (kGroups == 2 ? 5 * 128 * 4 : 0);
+  static constexpr int kSmem = kOffBar + 512;
+  static_assert(kSmem <= 227 * 1024 / kCtas - (kCtas - 1) * 512, "shared memory");
+  static constexpr uint32_t kTmem = HD == 256 || kCtas == 1 ? 512 : 256;
+  static constexpr uint32_t kColS = 0, kColO = 128;
+  static constexpr uint32_t kColQ = kQTmem ? 384 : 0;
+  static constexpr uint32_t kFmt = CT == CT_BF16 ? (1u << 7) | (1u << 10) : 0u;   // A, B bf16
+  static constexpr uint32_t kIdescQK = (1u << 4) | kFmt | (64u >> 3) << 17 | (128u >> 4) << 24;
+  static constexpr uint32_t kIdescPV = (1u << 4) | kFmt | (1u << 16) | static_cast<uint32_t>(HD >> 3) << 17 | (128u >> 4) << 24;
+};
+
+// sum over i < n of floor((a i + b) / m): the Euclid-like recursion, as a loop
+__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+  int64_t s = 0;
+  while (n > 0) {
+    if (a >= m) {
+      s += (n - 1) * n / 2 * (a / m);
+      a %= m;
+    }
+    if (b >= m) {
+      s += n * (b / m);
+      b %= m;
+    }
+    const int64_t y = a * n + b;
+    if (y < m) break;
+    n = y / m;
+    b = y % m;
+    const int64_t t = m;
+    m = a;
+    a = t;
+  }
+  return s;
+}
+
+__device__ __forceinline__ int tile_tokens(const AttnArgs& a) { return 128 / a.group; }
+__device__ __forceinline__ int tile_count(const AttnArgs& a, const Req& r) {
+  if (r.n < 1 || r.n * static_cast<int64_t>(a.group) <= a.rows_limit) return 0;
+  return (r.n + tile_tokens(a) - 1) / tile_tokens(a);
+}
+// keys that the last token of the tile sees
+__device__ __forceinline__ int tile_keys(const AttnArgs& a, const Req& r, int tile) {
+  const int64_t last = min(static_cast<int64_t>(tile + 1) * tile_tokens(a), static_cast<int64_t>(r.n));
+  return static_cast<int>(min(max(static_cast<int64_t>(r.kv) - r.n_all + last, static_cast<int64_t>(0)),
+                              static_cast<int64_t>(r.keys)));
+}
+__device__ __forceinline__ int tile_units(const AttnArgs& a, const Req& r, int tile) {
+  return max(1, (tile_keys(a, r, tile) + 63) >> 6);
+}
+// units of one KV head in the tiles before `tile`
+__device__ __forceinline__ int64_t units_before(const AttnArgs& a, const Req& r, int tile) {
+  const int64_t tt = tile_tokens(a), c = static_cast<int64_t>(r.kv) - r.n_all;
+  const int full = min(tile, r.n / static_cast<int>(tt));   // tiles with all their tokens
+  int64_t s = 0;
+  int i = 0;
+  if (c >= 0 && r.keys == r.kv) {   // ceil((c + (i + 1) tt) / 64), at least 1 since tt >= 1
+    s = floor_sum(full, 64, tt, c + tt + 63);
+    i = full;
+  }
+  for (; i < tile; ++i) s += tile_units(a, r, i);
+  return s;
+}
+
+// The helpers replace infinite and NaN values of V by 0 in the units that some rows do
+// not see whole (0 * inf in the product would reach those rows); this adds weight * value
+// of such keys to the rows that do see them.  Called by whole warps with O at rest; the
+// weights are the rounded ones of the product, from P in shared memory.
+template <int CT, int HD>
+__device__ __noinline__ void restore_bad_values(const AttnArgs& a, int b, int head, int k0, int keys, int lim,
+                                                const uint8_t* p_buf, int row, uint32_t o_tmem) {
+  constexpr bool BF = CT == CT_BF16;
+  for (int c = 0; c < HD / 32; ++c) {
+    uint32_t r[32];
+    tc_ld32(o_tmem + c * 32, r);
+    tc_wait_ld();
+    for (int j = 0; j < 64 && k0 + j < keys; ++j) {
+      const int key = k0 + j;
+      const int page = a.table[b * a.table_ld + (key >> a.shift)];
+      if (page < 0 || page >= a.c.pages) continue;
+      const int64_t in = key & (a.c.page_size - 1);
+      const int64_t at = page * a.c.v_stride[0] + head * a.c.v_stride[1] + in * a.c.v_stride[2] + c * 32;
+      const float p = unpack2<BF>(*reinterpret_cast<const uint16_t*>(p_buf + sw128(row, j >> 3) + (j & 7) * 2)).x;
+#pragma unroll
+      for (int x = 0; x < 32; ++x) {
+        uint32_t v;
+        if constexpr (CT == CT_Q8) {
+          const uint32_t s = static_cast<const uint16_t*>(
+              a.c.v_scale)[page * a.c.vs_stride[0] + head * a.c.vs_stride[1] + in * a.c.vs_stride[2] + c];
+          v = dq2(static_cast<const uint8_t*>(a.c.v)[at + x], 0x4040u, s | s << 16) & 0xFFFFu;
+        } else {
+          v = static_cast<const uint16_t*>(a.c.v)[at + x];
+        }
+        if (bad16<BF>(v) && key < lim) r[x] = __float_as_uint(__uint_as_float(r[x]) + p * unpack2<BF>(v).x);
+      }
+    }
+    __syncwarp();
+    tc_st32(o_tmem + c * 32, r);
+    tc_wait_st();
+  }
+}
+
+template <int CT, int HD>
+__global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::kCtas)
+    paged_tiles_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap k_map,
+                       const __grid_constant__ CUtensorMap v_map, uint32_t* err) {
+  using C = TilesCfg<CT, HD>;
+  constexpr bool BF = CT == CT_BF16, Q8 = C::kQ8;
+  static_assert(C::kColO + HD + (C::kQTmem ? C::kColQ - 384 + HD / 2 : 0) <= C::kTmem, "tensor memory");
+  constexpr int NH = C::kHelpers, RING = C::kRing, PB = C::kPBufs, NG = C::kGroups;
+  extern __shared__ __align__(1024) uint8_t sm[];
+  uint64_t* bar = reinterpret_cast<uint64_t*>(sm + C::kOffBar);
+  uint64_t* landed = bar;               // [RING or RAW] TMA -> MMA or helpers
+  uint64_t* raw_free = landed + 6;      // [RAW] helpers -> loader
+  uint64_t* full = raw_free + 6;        // [RING] helpers -> MMA
+  uint64_t* empty = full + 6;           // [RING] MMA -> loader or helpers
+  uint64_t* s_full = empty + 6;         // [2] QK -> softmax
+  uint64_t* s_free = s_full + 2;        // [2] softmax -> QK
+  uint64_t* p_full = s_free + 2;        // [2] softmax -> PV
+  uint64_t* pv_done = p_full + 2;       // [2] PV -> softmax
+  uint64_t* q_full = pv_done + 2;       // softmax -> QK: Q of the next item is in
+  uint64_t* o_free = q_full + 1;        // softmax -> PV: O of the last item is read
+  uint64_t* fix_req = o_free + 1;       // PV -> helpers: a V half to clean
+  uint64_t* fix_done = fix_req + 1;     // helpers -> PV
+  uint64_t* done = fix_done + 1;
+  uint64_t* m_full = done + 1;          // [4][2] between the groups' warps of the same rows: maximum of unit i
+  uint64_t* l_full = m_full + 8;        // [4] the same: both groups' sums of an item
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(l_full + 4);
+  volatile uint32_t* abort_flag = tmem_holder + 1;
+  // [8] by unit: unit + 1 if the helpers took a bad value out of its V (they are fewer than
+  // 8 units ahead of the softmax)
+  volatile int* bad = reinterpret_cast<int*>(tmem_holder + 2);
+  struct First {
+    int tile, head, u;
+  };
+  First* first_at = reinterpret_cast<First*>(tmem_holder + 10);
+  struct Fix {
+    int slot, valid, edge, unit;   // ring slot (-1: no more), keys of the unit that exist
+  };
+  Fix* fix = reinterpret_cast<Fix*>(tmem_holder + 14);
+  volatile float* m_sh = reinterpret_cast<float*>(sm + C::kOffX);   // [128]
+  volatile float* l_sh = m_sh + 128;                                 // [2 items][2 groups][128]
+  static_assert((4 * 6 + 25) * 8 + 14 * 4 + sizeof(Fix) <= 512 && RING <= 6 && C::kRaw <= 6, "barrier area");
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  griddep_launch_dependents();
+  const Start st = find_start<C::kThreads>(a, sm + C::kOffP, [&](int b) -> int64_t {
+    const Req r = get_req(a, b);
+    const int tiles = tile_count(a, r);
+    return tiles ? units_before(a, r, tiles) * a.c.kv_heads : 0;
+  });
+  if (tid == 0) a.desc[blockIdx.x] = make_int4(-1, -1, 0, 0);
+  const int n = static_cast<int>(st.u1 - st.u0);
+  if (n == 0) return;
+  const uint32_t sbase = smem_u32(sm);
+  if (sbase & 1023u) {   // the descriptors need the swizzle atoms' alignment
+    if (tid == 0) atomicOr(err, ERR_BAD_PARAM);
+    return;
+  }
+  if (warp == 0) {   // the tile, head and unit at which the range starts: a 32-way search
+    const Req r = get_req(a, st.b);
+    int lo = 0, hi = tile_count(a, r);   // units_before(lo) * heads <= local < units_before(hi) * heads
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 31) / 32, t = min(lo + lane * step, hi);
+      const bool le = t < hi && units_before(a, r, t) * a.c.kv_heads <= st.local;
+      const int k = 31 - __clz(__ballot_sync(0xffffffffu, le));   // lane 0 always holds
+      const int nlo = lo + k * step;
+      hi = min(hi, nlo + step);
+      lo = nlo;
+    }
+    if (lane == 0) {
+      const int64_t rest = st.local - units_before(a, r, lo) * a.c.kv_heads;
+      const int of = tile_units(a, r, lo);
+      *first_at = First{lo, static_cast<int>(rest / of), static_cast<int>(rest % of)};
+    }
+  }
+  if (tid == 0) {
+    for (int i = 0; i < 6; ++i) {
+      mbar_init(&landed[i], Q8 ? 33 : 1);   // int8: 32 lanes' copies of the scales as well
+      mbar_init(&raw_free[i], NH);
+      mbar_init(&full[i], NH);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 8; ++i) bad[i] = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_free[i], 4);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&pv_done[i], 1);
+    }
+    mbar_init(q_full, 4);
+    mbar_init(o_free, 4 * NG);
+    mbar_init(fix_req, 1);
+    mbar_init(fix_done, NH);
+    mbar_init(done, 2);
+    for (int i = 0; i < 8; ++i) mbar_init(&m_full[i], 1);
+    for (int i = 0; i < 4; ++i) mbar_init(&l_full[i], 2);
+    *abort_flag = 0u;
+    mbar_fence_init();
+  }
+  if (warp == C::kQkWarp) tc_alloc(tmem_holder, C::kTmem);
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = *tmem_holder;
+  auto fail = [&]() {
+    atomicOr(err, ERR_MBAR_TIMEOUT);
+    *abort_flag = 1u;
+  };
+
+  struct Pos {
+    int b, tile, head, u, of, tiles;
+    Req r;
+  };
+  Pos at;
+  at.b = st.b;
+  at.r = get_req(a, st.b);
+  at.tiles = tile_count(a, at.r);
+  at.tile = first_at->tile;
+  at.head = first_at->head;
+  at.u = first_at->u;
+  at.of = tile_units(a, at.r, at.tile);
+  // the next item (not called past the last unit of the launch)
+  auto next_item = [&](Pos& p) {
+    p.u = 0;
+    if (++p.head == a.c.kv_heads) {
+      p.head = 0;
+      if (++p.tile == p.tiles) {
+        p.tile = 0;
+        do {
+          if (++p.b >= a.n_req) return;
+          p.r = get_req(a, p.b);
+          p.tiles = tile_count(a, p.r);
+        } while (p.tiles == 0);
+      }
+      p.of = tile_units(a, p.r, p.tile);
+    }
+  };
+
+  // keys that every row of the item's tile sees; a unit past them needs care (is not seen
+  // whole by some row, or holds fewer than 64 keys)
+  auto seen_by_all = [&](const Pos& p) {
+    return max(0, min(p.r.keys, p.r.kv - p.r.n_all + p.tile * tile_tokens(a) + 1));
+  };
+
+  if (warp < 4 * NG) {
+    reg_inc<C::kRegsSoftmax>();
+    // ----------------------------------------------------------------- softmax
+    const int grp = NG == 2 ? warp >> 2 : 0, qd = warp & 3, row = qd * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(qd * 32) << 16;
+    const float sc = a.scale * 1.4426950408889634f;
+    const int tt = tile_tokens(a), t_in = row / a.group, hl = row - t_in * a.group;
+    bool ok = true;
+    auto load_q = [&](const Pos& p) {   // this row of Q (zero past the last row)
+      const int t = p.tile * tt + t_in;
+      const bool valid = t_in < tt && t < p.r.n;
+      const uint4* src = reinterpret_cast<const uint4*>(a.q + static_cast<int64_t>(p.r.q0 + t) * a.q_tok +
+                                                        (p.head * a.group + hl) * a.q_head);
+#pragma unroll 2
+      for (int c = 0; c < HD / 32; ++c) {
+        uint4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = valid ? __ldg(src + c * 4 + j) : make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (C::kQTmem) {
+          const uint32_t w[16] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w,
+                                  v[2].x, v[2].y, v[2].z, v[2].w, v[3].x, v[3].y, v[3].z, v[3].w};
+          tc_st16(tmem + lanes + C::kColQ + c * 16, w);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int ch = c * 4 + j;
+            *reinterpret_cast<uint4*>(sm + C::kOffQ + (ch >> 3) * 16384 + sw128(row, ch & 7)) = v[j];
+          }
+        }
+      }
+      if constexpr (C::kQTmem) {
+        tc_wait_st();
+        tc_before();
+      } else {
+        fence_proxy_async_smem();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    };
+    if (grp == 0) load_q(at);
+    int i = 0, item = 0;
+    while (i < n && ok && !*abort_flag) {
+      // one item, or this CTA's part of it: units i .. last
+      const int count = min(at.of - at.u, n - i), begin_i = i, last = i + count - 1;
+      const int t = at.tile * tt + t_in;
+      const bool valid = t_in < tt && t < at.r.n;
+      const int lim = valid ? max(0, min(at.r.keys, at.r.kv - at.r.n_all + t + 1)) : 0;   // keys < lim
+      const int all = seen_by_all(at);
+      const bool any = __any_sync(0xffffffffu, valid);   // a warp without rows only keeps the barriers going
+      // m_ref: the row's reference maximum as this group last knew it, its sum relative to it
+      float m_ref = -INFINITY, l_run = 0.f;
+      Pos next = at;
+      if (last + 1 < n) next_item(next);
+      for (; i <= last && ok; ++i) {
+        if (NG == 2 && (i & 1) != grp) continue;
+        const int b = i & 1, pb = PB == 2 ? b : 0, k0 = (at.u + i - begin_i) * 64;
+        if (!(ok = warp_wait(&s_full[b], (i >> 1) & 1))) break;
+        tc_after();
+        float s[64];
+        float mt = -INFINITY;
+        if (any) {
+          uint32_t r0[32], r1[32];
+          tc_ld32(tmem + lanes + C::kColS + b * 64, r0);
+          tc_ld32(tmem + lanes + C::kColS + b * 64 + 32, r1);
+          tc_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            s[j] = __uint_as_float(r0[j]);
+            s[32 + j] = __uint_as_float(r1[j]);
+          }
+        }
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[b]);
+        if (any) {
+          if (k0 + 64 > all) {
+            const int rem = lim - k0;
+#pragma unroll
+            for (int j = 0; j < 64; ++j) s[j] = j < rem ? s[j] : -INFINITY;
+          }
+          float mx[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mx[j] = fmaxf(s[j], s[4 + j]);
+#pragma unroll
+          for (int j = 8; j < 64; j += 8) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) mx[x] = fmaxf(mx[x], fmaxf(s[j + x], s[j + 4 + x]));
+          }
+          mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+        }
+        // the row's reference maximum after the unit before this one
+        float m_old = m_ref;
+        if (NG == 2 && i > 0) {
+          if (!(ok = warp_wait(&m_full[qd * 2 + (b ^ 1)], ((i - 1) >> 1) & 1))) break;
+          if (i > begin_i) m_old = m_sh[row];
+        }
+        const bool grows = mt > m_old + 8.f || (m_old == -INFINITY && mt > -INFINITY);
+        float m_new = m_old;
+        if (__any_sync(0xffffffffu, grows)) {
+          if (grows) m_new = mt;
+          if (i > begin_i) {
+            const float cor = m_old == m_new ? 1.f : ex2_approx(m_old - m_new);
+            if (!(ok = warp_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1))) break;   // O is at rest
+            tc_after();
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; ++c) {
+              uint32_t r[32];
+              tc_ld32(tmem + lanes + C::kColO + c * 32, r);
+              tc_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * cor);
+              tc_st32(tmem + lanes + C::kColO + c * 32, r);
+            }
+            tc_wait_st();
+          }
+        }
+        const bool edge = any && all < min(k0 + 64, at.r.keys);   // some row does not see the unit whole
+        if (NG == 2) {
+          m_sh[row] = m_new;
+          tc_before();
+          __syncwarp();
+          if (!edge && lane == 0) mbar_arrive(&m_full[qd * 2 + b]);   // (edge: below, when O is complete)
+        }
+        if (m_ref != m_new) {
+          l_run *= ex2_approx(m_ref - m_new);
+          m_ref = m_new;
+        }
+        const float off = m_ref == -INFINITY ? 0.f : -m_ref;
+        // the P buffer is free once the product that read it is done
+        if (i >= PB && !(ok = warp_wait(&pv_done[(i - PB) & 1], ((i - PB) >> 1) & 1))) break;
+        if (any) {
+          float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              // 2^(scale log2(e) s - m): one fma and one ex2; a masked key's -inf gives 0
+              w[j] = pack2<BF>(ex2_approx(fmaf(s[8 * c + 2 * j], sc, off)), ex2_approx(fmaf(s[8 * c + 2 * j + 1], sc, off)));
+              const float2 p = unpack2<BF>(w[j]);   // the rounded weights are summed: see the rows form
+              sums[j] += p.x + p.y;
+            }
+            *reinterpret_cast<uint4*>(sm + C::kOffP + pb * C::kPBytes + sw128(row, c)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          l_run += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        }
+        fence_proxy_async_smem();
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[b]);
+        // Q of the next item may follow once every S of this one is made
+        if (i == last && i + 1 < n) load_q(next);
+        if (edge) {
+          // bad values that the helpers took out of V, for the rows that see them
+          if (!(ok = warp_wait(&pv_done[b], (i >> 1) & 1))) break;
+          tc_after();
+          if (bad[i & 7] == i + 1)
+            restore_bad_values<CT, HD>(a, at.b, at.head, k0, at.r.keys, lim, sm + C::kOffP + pb * C::kPBytes, row,
+                                       tmem + lanes + C::kColO);
+          tc_before();
+          __syncwarp();
+          if (NG == 2 && lane == 0) mbar_arrive(&m_full[qd * 2 + b]);
+        }
+      }
+      if (!ok) break;
+      // the item's rows, or this part's; two groups take half of the columns each
+      if (NG == 2) {
+        if ((last & 1) != grp) {
+          if (!(ok = warp_wait(&m_full[qd * 2 + (last & 1)], (last >> 1) & 1))) break;
+          const float m_end = m_sh[row];
+          if (m_ref != m_end) {
+            l_run *= ex2_approx(m_ref - m_end);
+            m_ref = m_end;
+          }
+        }
+        volatile float* l2 = l_sh + (item & 1) * 256;
+        l2[grp * 128 + row] = l_run;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&l_full[qd]);
+        if (!(ok = warp_wait(&l_full[qd], item & 1))) break;
+        l_run = l2[row] + l2[128 + row];
+      }
+      if (!(ok = warp_wait(&pv_done[last & 1], (last >> 1) & 1))) break;
+      tc_after();
+      const int64_t begin = st.u0 + begin_i - at.u, end = begin + at.of;   // the item's units
+      const bool whole = begin >= st.u0 && end <= st.u1;
+      const int slot = 2 * blockIdx.x + (begin > st.u0 ? 1 : 0);
+      if (tid == 0 && begin >= st.u0 && !whole)
+        a.desc[blockIdx.x] = make_int4(slot, range_of(st.units, end - 1, st.ctas), at.b << 10 | at.head, at.tile);
+      if (any) {
+        const bool sees = lim > 0;
+        const float inv = 1.f / l_run;
+        const int64_t tok = at.r.q0 + t;
+        const int head = at.head * a.group + hl;
+#pragma unroll 1
+        for (int c = grp * (HD / 32 / NG); c < (grp + 1) * (HD / 32 / NG); ++c) {
+          uint4 gv[4];
+          if (whole && a.gate && valid) {
+            const uint4* gp = reinterpret_cast<const uint4*>(a.gate + tok * a.g_tok + head * a.g_head + c * 32);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) gv[j] = __ldg(gp + j);
+          }
+          uint32_t r[32];
+          tc_ld32(tmem + lanes + C::kColO + c * 32, r);
+          tc_wait_ld();
+          if (!valid) continue;
+          if (!whole) {
+            float4* dst = reinterpret_cast<float4*>(a.part + (static_cast<int64_t>(slot) * 128 + row) * HD + c * 32);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              dst[j] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
+                                   __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
+          } else {
+            uint4* dst = reinterpret_cast<uint4*>(a.out + tok * a.o_tok + head * a.o_head + c * 32);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              float v[8];
+#pragma unroll
+              for (int x = 0; x < 8; ++x) v[x] = sees ? __uint_as_float(r[8 * j + x]) * inv : 0.f;
+              if (a.gate) {
+                const uint32_t gw[4] = {gv[j].x, gv[j].y, gv[j].z, gv[j].w};
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                  const float2 y = unpack2<BF>(gw[x]);
+                  v[2 * x] = gated(v[2 * x], y.x);
+                  v[2 * x + 1] = gated(v[2 * x + 1], y.y);
+                }
+              }
+              dst[j] = make_uint4(pack2<BF>(v[0], v[1]), pack2<BF>(v[2], v[3]), pack2<BF>(v[4], v[5]), pack2<BF>(v[6], v[7]));
+            }
+          }
+        }
+        if (!whole && valid && grp == 0) a.ml[slot * 128 + row] = make_float2(m_ref, l_run);
+      }
+      tc_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(o_free);
+      at = next;
+      ++item;
+    }
+    if (!ok) fail();
+  } else {
+    reg_dec<C::kRegsOther>();
+    if (warp == C::kQkWarp) {
+      // --------------------------------------------------------------- S = Q K^T
+      if (lane == 0) {
+        bool ok = true;
+        int left = min(at.of - at.u, n), item = 0;
+        bool starts = true;
+        for (int i = 0; i < n && ok && !*abort_flag; ++i) {
+          // K(i) follows i Ks and the Vs before V(i - 1), which it precedes unless it starts an item
+          const int h = 2 * i - (starts ? 0 : 1), slot = h % RING, b = i & 1;
+          if (starts && !(ok = tc_wait(q_full, item & 1))) break;
+          if (!(ok = tc_wait(Q8 ? &full[slot] : &landed[slot], (h / RING) & 1))) break;
+          if (!(ok = tc_wait(&s_free[b], ((i >> 1) & 1) ^ 1))) break;
+          tc_after();
+          const uint64_t kd = sw128_desc(sbase + slot * C::kHalf);
+          const uint64_t qd = C::kQTmem ? 0ull : sw128_desc(sbase + C::kOffQ);
+#pragma unroll
+          for (int s = 0; s < HD / 16; ++s) {
+            const uint64_t bd = kd + ((s >> 2) * 8192 + (s & 3) * 32) / 16;   // the address field, in 16-byte units
+            if constexpr (C::kQTmem)
+              tc_mma_ts(tmem + C::kColS + b * 64, tmem + C::kColQ + s * 8, bd, C::kIdescQK, s > 0 ? 1u : 0u);
+            else
+              tc_mma(tmem + C::kColS + b * 64, qd + ((s >> 2) * 16384 + (s & 3) * 32) / 16, bd, C::kIdescQK, s > 0 ? 1u : 0u);
+          }
+          tc_commit(&s_full[b]);
+          tc_commit(&empty[slot]);
+          starts = --left == 0;
+          if (starts && i + 1 < n) {
+            next_item(at);
+            left = at.of;
+            ++item;
+          }
+        }
+        if (!ok) fail();
+        tc_commit(done);   // every issued MMA has completed before tensor memory is released
+        if (!tc_wait(done, 0)) fail();
+      }
+    } else if (warp == C::kPvWarp) {
+      // ---------------------------------------------------------------- O += P V
+      if (lane == 0) {
+        bool ok = true;
+        int left = min(at.of - at.u, n), item = 0, fixes = 0, all = seen_by_all(at);
+        bool starts = true;
+        for (int i = 0; i < n && ok && !*abort_flag; ++i) {
+          // V(i) follows i Vs and i + 1 Ks, and K(i + 1) unless unit i ends an item
+          const int h = 2 * i + 1 + (left != 1 && i + 1 < n ? 1 : 0), slot = h % RING, pb = PB == 2 ? i & 1 : 0;
+          if (starts && item > 0 && !(ok = tc_wait(o_free, (item - 1) & 1))) break;
+          if (!(ok = tc_wait(Q8 ? &full[slot] : &landed[slot], (h / RING) & 1))) break;
+          if (!Q8 && at.u * 64 + 64 > all) {
+            *fix = Fix{slot, at.r.keys - at.u * 64, all < min(at.u * 64 + 64, at.r.keys), i};
+            mbar_arrive(fix_req);
+            if (!(ok = tc_wait(fix_done, fixes++ & 1))) break;
+          }
+          if (!(ok = tc_wait(&p_full[i & 1], (i >> 1) & 1))) break;
+          tc_after();
+          const uint64_t pd = sw128_desc(sbase + C::kOffP + pb * C::kPBytes);
+          const uint64_t vd = sw128_desc_mn(sbase + slot * C::kHalf, 8192);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc_mma(tmem + C::kColO, pd + k * 2, vd + k * 128, C::kIdescPV, (!starts || k > 0) ? 1u : 0u);
+          tc_commit(&pv_done[i & 1]);
+          tc_commit(&empty[slot]);
+          ++at.u;
+          starts = --left == 0;
+          if (starts && i + 1 < n) {
+            next_item(at);
+            left = at.of;
+            all = seen_by_all(at);
+            ++item;
+          }
+        }
+        if (!ok) fail();
+        if constexpr (!Q8) {
+          fix->slot = -1;
+          mbar_arrive(fix_req);
+        }
+        tc_commit(done);
+        if (!tc_wait(done, 0)) fail();
+      }
+    } else if (warp == C::kLoadWarp) {
+      // ------------------------------------------------------------------ loader
+      // Halves in MMA order: per unit K(i) then V(i - 1), or V(i - 1) first where unit i
+      // starts an item.  A lane owns one TMA box of a half: 64 dims (int8: all) of the keys
+      // of one page.
+      constexpr int ATOMS = Q8 ? 1 : HD / 64, LR = Q8 ? C::kRaw : RING;
+      const int rows = min(a.c.page_size, 64), part = lane / ATOMS, atom = lane % ATOMS;
+      const bool mine = part * rows < 64;
+      auto page_of = [&](const Pos& p) -> int {   // -1: outside the pool, read as 0
+        const int key = p.u * 64 + part * rows;
+        return mine && key < p.r.keys ? a.table[p.b * a.table_ld + (key >> a.shift)] : -1;
+      };
+      int h = 0;
+      bool ok = true;
+      auto load = [&](bool v, int page, int u, int head, int keys) {
+        const int slot = h % LR;
+        if (!(ok = warp_wait(Q8 ? &raw_free[slot] : &empty[slot], ((h / LR) & 1) ^ 1))) return;
+        if (lane == 0) mbar_arrive_expect_tx(&landed[slot], Q8 ? C::kRawHalf : C::kHalf);
+        __syncwarp();
+        const int in = (u * 64 + part * rows) & (a.c.page_size - 1);
+        uint8_t* dst = Q8 ? sm + C::kOffRaw + slot * C::kRawBytes + part * rows * HD
+                          : sm + slot * C::kHalf + atom * 8192 + part * rows * 128;
+        if (mine) tma_load_4d(dst, v ? &v_map : &k_map, atom * 64, in, head, page, &landed[slot]);
+        if constexpr (Q8) {
+          const uint16_t* sc = static_cast<const uint16_t*>(v ? a.c.v_scale : a.c.k_scale);
+          const int64_t* ss = v ? a.c.vs_stride : a.c.ks_stride;
+          const uint32_t sb = sbase + C::kOffRaw + slot * C::kRawBytes + C::kRawHalf;
+  #pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int k = x * 32 + lane, key = u * 64 + k;
+            const int pg = __shfl_sync(0xffffffffu, page, k / rows);
+            const bool in_pool = key < keys && pg >= 0 && pg < a.c.pages;
+            const uint16_t* src = in_pool ? sc + pg * ss[0] + head * ss[1] + (key & (a.c.page_size - 1)) * ss[2] : sc;
+            cp_async_small<HD / 16>(sb + k * (HD / 16), src, in_pool);
+          }
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(smem_u32(&landed[slot])) : "memory");
+        }
+        ++h;
+      };
+      int pk = page_of(at), pv = -1, u_v = 0, head_v = 0, keys_v = 0, left = min(at.of - at.u, n);
+      bool starts = true;
+      for (int i = 0; i <= n && ok && !*abort_flag; ++i) {
+        if (i > 0 && (starts || i == n)) load(true, pv, u_v, head_v, keys_v);
+        if (i == n || !ok) break;
+        load(false, pk, at.u, at.head, at.r.keys);
+        if (i > 0 && !starts && ok) load(true, pv, u_v, head_v, keys_v);
+        pv = pk;
+        u_v = at.u;
+        head_v = at.head;
+        keys_v = at.r.keys;
+        starts = --left == 0;
+        if (i + 1 < n) {
+          if (starts) {
+            next_item(at);
+            left = at.of;
+          } else {
+            ++at.u;
+          }
+          pk = page_of(at);   // in flight while the ring is full
+        }
+      }
+      if (!ok) fail();
+      if (!ok || *abort_flag) {   // no copy may still be in flight when the CTA ends
+        if constexpr (Q8) cp_async_wait_all();
+        for (int f = max(0, h - LR); f < h; ++f) tc_wait(&landed[f % LR], (f / LR) & 1);
+      }
+    } else if (warp >= C::kHelpFirst) {
+      // ----------------------------------------------------------------- helpers
+      const int hw = warp - C::kHelpFirst;
+      bool ok = true;
+      if constexpr (!Q8) {
+        for (int k = 0; ok && !*abort_flag; ++k) {
+          if (!(ok = warp_wait(fix_req, k & 1))) break;
+          const Fix f = *fix;
+          if (f.slot < 0) break;
+          uint8_t* hb = sm + f.slot * C::kHalf;
+          bool any_bad = false;
+          for (int idx = hw * 32 + lane; idx < 64 * HD / 8; idx += NH * 32) {
+            const int key = idx / (HD / 8), ch = idx % (HD / 8);
+            uint4* p = reinterpret_cast<uint4*>(hb + (ch >> 3) * 8192 + sw128(key, ch & 7));
+            if (key >= f.valid) {
+              *p = make_uint4(0u, 0u, 0u, 0u);
+            } else if (f.edge) {
+              const uint4 x = *p;
+              uint32_t w[4] = {x.x, x.y, x.z, x.w};
+              if (drop_bad<BF>(w[0]) | drop_bad<BF>(w[1]) | drop_bad<BF>(w[2]) | drop_bad<BF>(w[3])) {
+                *p = make_uint4(w[0], w[1], w[2], w[3]);
+                any_bad = true;
+              }
+            }
+          }
+          if (any_bad) bad[f.unit & 7] = f.unit + 1;
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(fix_done);
+        }
+      } else {
+        constexpr int CPK = HD / 16;   // 16-byte chunks of a cached row
+        int h = 0;
+        auto convert = [&](bool v, int valid, bool edge, int unit) {
+          const int slot = h % RING, rs = h % C::kRaw;
+          if (!(ok = warp_wait(&landed[rs], (h / C::kRaw) & 1)) || !(ok = warp_wait(&empty[slot], ((h / RING) & 1) ^ 1))) return;
+          const uint8_t* raw = sm + C::kOffRaw + rs * C::kRawBytes;
+          bool any_bad = false;
+          constexpr int PER = 64 * CPK / (NH * 32), BATCH = PER > 4 ? 4 : PER;
+          static_assert(PER * NH * 32 == 64 * CPK, "the helpers' shares");
+  #pragma unroll 1
+          for (int x0 = 0; x0 < PER; x0 += BATCH) {
+            uint4 x[BATCH];
+            uint32_t sc[BATCH];
+  #pragma unroll
+            for (int x1 = 0; x1 < BATCH; ++x1) {   // 16 dims: 16-bit chunks 2 ch and 2 ch + 1
+              const int idx = (x0 + x1) * NH * 32 + hw * 32 + lane, key = idx / CPK, ch = idx % CPK;
+              x[x1] = *reinterpret_cast<const uint4*>(raw + idx * 16);
+              sc[x1] = *reinterpret_cast<const uint16_t*>(raw + C::kRawHalf + key * (HD / 16) + (ch >> 1) * 2);
+              if (key >= valid) sc[x1] = 0u;   // rows past the last key: +-0
+            }
+  #pragma unroll
+            for (int x1 = 0; x1 < BATCH; ++x1) {
+              const int idx = (x0 + x1) * NH * 32 + hw * 32 + lane, key = idx / CPK, ch = idx % CPK;
+              const uint32_t s2 = sc[x1] | sc[x1] << 16;
+              const uint32_t in[4] = {x[x1].x, x[x1].y, x[x1].z, x[x1].w};
+              uint32_t o[8];
+  #pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                o[2 * y] = dq2(in[y], 0x5140u, s2);
+                o[2 * y + 1] = dq2(in[y], 0x7362u, s2);
+              }
+              if (edge) {
+  #pragma unroll
+                for (int y = 0; y < 8; ++y) any_bad |= drop_bad<false>(o[y]);
+              }
+              // lanes of neighbouring atoms write their two chunks in opposite order: all banks once
+              const int first = (ch >> 2) & 1;
+              uint8_t* hb = sm + slot * C::kHalf + (ch >> 2) * 8192;
+              const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
+              *reinterpret_cast<uint4*>(hb + sw128(key, ((2 * ch) & 7) + first)) = first ? hi : lo;
+              *reinterpret_cast<uint4*>(hb + sw128(key, ((2 * ch) & 7) + (first ^ 1))) = first ? lo : hi;
+            }
+          }
+          if (any_bad) bad[unit & 7] = unit + 1;
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&full[slot]);
+            mbar_arrive(&raw_free[rs]);
+          }
+          ++h;
+        };
+        bool starts = true, edge_v = false;
+        int valid_v = 0, left = min(at.of - at.u, n);
+        for (int i = 0; i <= n && ok && !*abort_flag; ++i) {
+          if (i > 0 && (starts || i == n)) convert(true, valid_v, edge_v, i - 1);
+          if (i == n || !ok) break;
+          convert(false, at.r.keys - at.u * 64, false, i);
+          if (i > 0 && !starts && ok) convert(true, valid_v, edge_v, i - 1);
+          valid_v = at.r.keys - at.u * 64;
+          edge_v = seen_by_all(at) < min(at.u * 64 + 64, at.r.keys);
+          starts = --left == 0;
+          if (i + 1 < n) {
+            if (starts) {
+              next_item(at);
+              left = at.of;
+            } else {
+              ++at.u;
+            }
+          }
+        }
+      }
+      if (!ok) fail();
+    }
+  }
+
+  tc_before();
+  __syncthreads();
+  if (warp == C::kQkWarp) {
+    tc_after();
+    tc_dealloc(tmem, C::kTmem);
+  }
+}
+
+// The pool as TMA sees it: [page][head][slot][dim], a box of 64 dims (int8: the row) of the
+// keys of one page that fall in a unit of 64.  A dimension of one entry takes any stride.
+bool page_map(CUtensorMap* map, const tlx_paged_kv& c, const void* base, const int64_t* stride) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static Encode enc = nullptr;   // looked up through the runtime: the library does not link the driver's
+  if (!enc) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return false;
+    enc = reinterpret_cast<Encode>(fn);
+  }
+  const bool q8 = c.dtype == TLX_DT_Q8;
+  const cuuint64_t esz = q8 ? 1 : 2;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.head_dim), static_cast<cuuint64_t>(c.page_size),
+                              static_cast<cuuint64_t>(c.kv_heads), static_cast<cuuint64_t>(c.pages)};
+  cuuint64_t strides[3];
+  for (int i = 0; i < 3; ++i)
+    strides[i] = dims[i + 1] > 1 ? static_cast<cuuint64_t>(stride[2 - i]) * esz : static_cast<cuuint64_t>(c.head_dim) * esz;
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(q8 ? c.head_dim : 64), static_cast<cuuint32_t>(std::min(c.page_size, 64)),
+                             1u, 1u};
+  const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+  return enc(map, q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims,
+             strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             q8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int CT, int HD>
+int launch_tiles(AttnArgs a, void* ws, int sms, cudaStream_t s) {
+  using C = TilesCfg<CT, HD>;
+  static bool configured = false;
+  if (!configured) {
+    if (cudaFuncSetAttribute(paged_tiles_kernel<CT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) !=
+        cudaSuccess)
+      return TLX_ERR_LAUNCH;
+    configured = true;
+  }
+  const int ctas = sms * C::kCtas;
+  set_split(a, ws, split_area(ctas, 128, HD));
+  a.by_item = 0;
+  CUtensorMap km, vm;
+  if (!page_map(&km, a.c, a.c.k, a.c.k_stride) || !page_map(&vm, a.c, a.c.v, a.c.v_stride)) return TLX_ERR_LAUNCH;
+  paged_tiles_kernel<CT, HD><<<ctas, C::kThreads, C::kSmem, s>>>(a, km, vm, static_cast<uint32_t*>(ws));
+  if (cudaGetLastError() != cudaSuccess) return TLX_ERR_LAUNCH;
+  return launch_combine(a, CT == CT_BF16, 128, ctas, 16, s);
+}
+
+}  // namespace
+
+int launch_paged_tiles(const AttnArgs& a, int ct, void* ws, int sms, cudaStream_t s) {
+  const int hd = a.c.head_dim;
+  if (ct == CT_F16) return hd == 256 ? launch_tiles<CT_F16, 256>(a, ws, sms, s) : hd == 128 ? launch_tiles<CT_F16, 128>(a, ws, sms, s) : launch_tiles<CT_F16, 64>(a, ws, sms, s);
+  if (ct == CT_BF16) return hd == 256 ? launch_tiles<CT_BF16, 256>(a, ws, sms, s) : hd == 128 ? launch_tiles<CT_BF16, 128>(a, ws, sms, s) : launch_tiles<CT_BF16, 64>(a, ws, sms, s);
+  return hd == 256 ? launch_tiles<CT_Q8, 256>(a, ws, sms, s) : hd == 128 ? launch_tiles<CT_Q8, 128>(a, ws, sms, s) : launch_tiles<CT_Q8, 64>(a, ws, sms, s);
+}
+
+size_t paged_tiles_bytes(int hd, int sms) { return split_area(sms * (hd == 256 ? 1 : 2), 128, hd).end; }   // kCtas at most
+
+}  // namespace tlx
