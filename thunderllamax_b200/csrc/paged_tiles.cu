@@ -28,6 +28,10 @@ namespace {
 //                into fp16(code * scale)
 // Every wait is bounded: a timeout raises the error word, all roles leave, issued MMAs
 // and copies are drained and tensor memory is freed.
+//
+// Code size: the roles' loops run side by side on each scheduler, one warp each, so what
+// does not fit the instruction caches is fetched again for every unit.  Hence the loops
+// that could be unrolled further and are not, and one call site for each large body.
 template <int N>
 __device__ __forceinline__ void reg_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N));
@@ -381,37 +385,31 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
         const int b = i & 1, pb = PB == 2 ? b : 0, k0 = (at.u + i - begin_i) * 64;
         if (!(ok = warp_wait(&s_full[b], (i >> 1) & 1))) break;
         tc_after();
-        float s[64];
+        // Two passes over the unit's scores, 32 columns at a time: they stay in tensor memory
+        // between the maximum and the exponentials, which halves the registers and the code.
+        const int rem = lim - k0;
+        const bool cut = k0 + 64 > all;   // some row does not see the whole unit
         float mt = -INFINITY;
         if (any) {
-          uint32_t r0[32], r1[32];
-          tc_ld32(tmem + lanes + C::kColS + b * 64, r0);
-          tc_ld32(tmem + lanes + C::kColS + b * 64 + 32, r1);
-          tc_wait_ld();
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            uint32_t r[32];
+            tc_ld32(tmem + lanes + C::kColS + b * 64 + c * 32, r);
+            tc_wait_ld();
+            if (cut) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            s[j] = __uint_as_float(r0[j]);
-            s[32 + j] = __uint_as_float(r1[j]);
+              for (int j = 0; j < 32; ++j) r[j] = c * 32 + j < rem ? r[j] : 0xFF800000u;
+            }
+            float mx[4] = {mt, mt, mt, mt};
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) {
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                mx[x] = fmaxf(mx[x], fmaxf(__uint_as_float(r[j + x]), __uint_as_float(r[j + 4 + x])));
+            }
+            mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           }
-        }
-        tc_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[b]);
-        if (any) {
-          if (k0 + 64 > all) {
-            const int rem = lim - k0;
-#pragma unroll
-            for (int j = 0; j < 64; ++j) s[j] = j < rem ? s[j] : -INFINITY;
-          }
-          float mx[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) mx[j] = fmaxf(s[j], s[4 + j]);
-#pragma unroll
-          for (int j = 8; j < 64; j += 8) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x) mx[x] = fmaxf(mx[x], fmaxf(s[j + x], s[j + 4 + x]));
-          }
-          mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+          mt *= sc;
         }
         // the row's reference maximum after the unit before this one
         float m_old = m_ref;
@@ -455,24 +453,39 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
         if (i >= PB && !(ok = warp_wait(&pv_done[(i - PB) & 1], ((i - PB) >> 1) & 1))) break;
         if (any) {
           float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            uint32_t r[32];
+            tc_ld32(tmem + lanes + C::kColS + b * 64 + c * 32, r);
+            tc_wait_ld();
+            if (cut) {
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              // 2^(scale log2(e) s - m): one fma and one ex2; a masked key's -inf gives 0
-              w[j] = pack2<BF>(ex2_approx(fmaf(s[8 * c + 2 * j], sc, off)), ex2_approx(fmaf(s[8 * c + 2 * j + 1], sc, off)));
-              const float2 p = unpack2<BF>(w[j]);   // the rounded weights are summed: see the rows form
-              sums[j] += p.x + p.y;
+              for (int j = 0; j < 32; ++j) r[j] = c * 32 + j < rem ? r[j] : 0xFF800000u;
             }
-            *reinterpret_cast<uint4*>(sm + C::kOffP + pb * C::kPBytes + sw128(row, c)) = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              uint32_t w[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                // 2^(scale log2(e) s - m): one fma and one ex2; a masked key's -inf gives 0
+                w[j] = pack2<BF>(ex2_approx(fmaf(__uint_as_float(r[8 * x + 2 * j]), sc, off)),
+                                 ex2_approx(fmaf(__uint_as_float(r[8 * x + 2 * j + 1]), sc, off)));
+                const float2 p = unpack2<BF>(w[j]);   // the rounded weights are summed: see the rows form
+                sums[j] += p.x + p.y;
+              }
+              *reinterpret_cast<uint4*>(sm + C::kOffP + pb * C::kPBytes + sw128(row, c * 4 + x)) =
+                  make_uint4(w[0], w[1], w[2], w[3]);
+            }
           }
           l_run += (sums[0] + sums[1]) + (sums[2] + sums[3]);
         }
         fence_proxy_async_smem();
         tc_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[b]);
+        if (lane == 0) {
+          mbar_arrive(&p_full[b]);
+          mbar_arrive(&s_free[b]);
+        }
         // Q of the next item may follow once every S of this one is made
         if (i == last && i + 1 < n) load_q(next);
         if (edge) {
@@ -581,13 +594,16 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
           tc_after();
           const uint64_t kd = sw128_desc(sbase + slot * C::kHalf);
           const uint64_t qd = C::kQTmem ? 0ull : sw128_desc(sbase + C::kOffQ);
+#pragma unroll 1
+          for (int x = 0; x < HD / 64; ++x) {   // (a loop over the atoms: see the note on code size)
 #pragma unroll
-          for (int s = 0; s < HD / 16; ++s) {
-            const uint64_t bd = kd + ((s >> 2) * 8192 + (s & 3) * 32) / 16;   // the address field, in 16-byte units
-            if constexpr (C::kQTmem)
-              tc_mma_ts(tmem + C::kColS + b * 64, tmem + C::kColQ + s * 8, bd, C::kIdescQK, s > 0 ? 1u : 0u);
-            else
-              tc_mma(tmem + C::kColS + b * 64, qd + ((s >> 2) * 16384 + (s & 3) * 32) / 16, bd, C::kIdescQK, s > 0 ? 1u : 0u);
+            for (int y = 0; y < 4; ++y) {
+              const uint64_t bd = kd + (x * 8192 + y * 32) / 16;   // the address field, in 16-byte units
+              if constexpr (C::kQTmem)
+                tc_mma_ts(tmem + C::kColS + b * 64, tmem + C::kColQ + x * 32 + y * 8, bd, C::kIdescQK, x + y > 0 ? 1u : 0u);
+              else
+                tc_mma(tmem + C::kColS + b * 64, qd + (x * 16384 + y * 32) / 16, bd, C::kIdescQK, x + y > 0 ? 1u : 0u);
+            }
           }
           tc_commit(&s_full[b]);
           tc_commit(&empty[slot]);
@@ -658,7 +674,8 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
       };
       int h = 0;
       bool ok = true;
-      auto load = [&](bool v, int page, int u, int head, int keys) {
+      auto load = [&](bool v, const auto& x) {
+        const int page = x.page, u = x.u, head = x.head, keys = x.keys;
         const int slot = h % LR;
         if (!(ok = warp_wait(Q8 ? &raw_free[slot] : &empty[slot], ((h / LR) & 1) ^ 1))) return;
         if (lane == 0) mbar_arrive_expect_tx(&landed[slot], Q8 ? C::kRawHalf : C::kHalf);
@@ -683,26 +700,33 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
         }
         ++h;
       };
-      int pk = page_of(at), pv = -1, u_v = 0, head_v = 0, keys_v = 0, left = min(at.of - at.u, n);
+      struct Half {
+        int page, u, head, keys;
+      };
+      auto half_of = [&](const Pos& p) { return Half{page_of(p), p.u, p.head, p.r.keys}; };
+      // i Ks are out and v Vs; K(i) is next unless two Vs are owed, or one and unit i starts an item
+      Half k = half_of(at), v1{}, v2{};
+      int i = 0, v = 0, left = min(at.of - at.u, n);
       bool starts = true;
-      for (int i = 0; i <= n && ok && !*abort_flag; ++i) {
-        if (i > 0 && (starts || i == n)) load(true, pv, u_v, head_v, keys_v);
-        if (i == n || !ok) break;
-        load(false, pk, at.u, at.head, at.r.keys);
-        if (i > 0 && !starts && ok) load(true, pv, u_v, head_v, keys_v);
-        pv = pk;
-        u_v = at.u;
-        head_v = at.head;
-        keys_v = at.r.keys;
+      while (v < n && ok && !*abort_flag) {
+        const bool is_v = i - v == 2 || (i - v == 1 && (starts || i == n));
+        load(is_v, is_v ? (i - v == 2 ? v2 : v1) : k);
+        if (is_v) {
+          ++v;
+          continue;
+        }
+        ++i;
+        v2 = v1;
+        v1 = k;
         starts = --left == 0;
-        if (i + 1 < n) {
+        if (i < n) {
           if (starts) {
             next_item(at);
             left = at.of;
           } else {
             ++at.u;
           }
-          pk = page_of(at);   // in flight while the ring is full
+          k = half_of(at);   // the page id is in flight while the ring is full
         }
       }
       if (!ok) fail();
@@ -743,12 +767,12 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
       } else {
         constexpr int CPK = HD / 16;   // 16-byte chunks of a cached row
         int h = 0;
-        auto convert = [&](bool v, int valid, bool edge, int unit) {
+        auto convert = [&](int valid, bool edge, int unit) {
           const int slot = h % RING, rs = h % C::kRaw;
           if (!(ok = warp_wait(&landed[rs], (h / C::kRaw) & 1)) || !(ok = warp_wait(&empty[slot], ((h / RING) & 1) ^ 1))) return;
           const uint8_t* raw = sm + C::kOffRaw + rs * C::kRawBytes;
           bool any_bad = false;
-          constexpr int PER = 64 * CPK / (NH * 32), BATCH = PER > 4 ? 4 : PER;
+          constexpr int PER = 64 * CPK / (NH * 32), BATCH = PER > 2 ? 2 : PER;
           static_assert(PER * NH * 32 == 64 * CPK, "the helpers' shares");
   #pragma unroll 1
           for (int x0 = 0; x0 < PER; x0 += BATCH) {
@@ -793,23 +817,35 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
           }
           ++h;
         };
-        bool starts = true, edge_v = false;
-        int valid_v = 0, left = min(at.of - at.u, n);
-        for (int i = 0; i <= n && ok && !*abort_flag; ++i) {
-          if (i > 0 && (starts || i == n)) convert(true, valid_v, edge_v, i - 1);
-          if (i == n || !ok) break;
-          convert(false, at.r.keys - at.u * 64, false, i);
-          if (i > 0 && !starts && ok) convert(true, valid_v, edge_v, i - 1);
-          valid_v = at.r.keys - at.u * 64;
-          edge_v = seen_by_all(at) < min(at.u * 64 + 64, at.r.keys);
+        struct Half {
+          int valid, edge;
+        };
+        auto half_of = [&](const Pos& p) {
+          return Half{p.r.keys - p.u * 64, seen_by_all(p) < min(p.u * 64 + 64, p.r.keys)};
+        };
+        Half k = half_of(at), v1{}, v2{};   // order of the halves: see the loader
+        int i = 0, v = 0, left = min(at.of - at.u, n);
+        bool starts = true;
+        while (v < n && ok && !*abort_flag) {
+          const bool is_v = i - v == 2 || (i - v == 1 && (starts || i == n));
+          const Half x = is_v ? (i - v == 2 ? v2 : v1) : k;
+          convert(x.valid, is_v && x.edge, v);
+          if (is_v) {
+            ++v;
+            continue;
+          }
+          ++i;
+          v2 = v1;
+          v1 = k;
           starts = --left == 0;
-          if (i + 1 < n) {
+          if (i < n) {
             if (starts) {
               next_item(at);
               left = at.of;
             } else {
               ++at.u;
             }
+            k = half_of(at);
           }
         }
       }
