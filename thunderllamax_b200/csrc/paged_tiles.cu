@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
       mbar_init(&p_full[i], 4);
       mbar_init(&pv_done[i], 1);
     }
-    mbar_init(q_full, 4);
+    mbar_init(q_full, 4 * NG);
     mbar_init(o_free, 4 * NG);
     mbar_init(fix_req, 1);
     mbar_init(fix_done, NH);
@@ -340,21 +340,24 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
       const bool valid = t_in < tt && t < p.r.n;
       const uint4* src = reinterpret_cast<const uint4*>(a.q + static_cast<int64_t>(p.r.q0 + t) * a.q_tok +
                                                         (p.head * a.group + hl) * a.q_head);
-#pragma unroll 2
-      for (int c = 0; c < HD / 32; ++c) {
-        uint4 v[4];
+      constexpr int CH = HD / 8 / NG, FLY = CH < 8 ? CH : 8;   // 16-byte chunks of this group, FLY in flight
+#pragma unroll 1
+      for (int c0 = grp * CH; c0 < (grp + 1) * CH; c0 += FLY) {
+        uint4 v[FLY];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = valid ? __ldg(src + c * 4 + j) : make_uint4(0u, 0u, 0u, 0u);
+        for (int j = 0; j < FLY; ++j) v[j] = valid ? __ldg(src + c0 + j) : make_uint4(0u, 0u, 0u, 0u);
         if constexpr (C::kQTmem) {
-          const uint32_t w[16] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w,
-                                  v[2].x, v[2].y, v[2].z, v[2].w, v[3].x, v[3].y, v[3].z, v[3].w};
-          tc_st16(tmem + lanes + C::kColQ + c * 16, w);
+#pragma unroll
+          for (int x = 0; x < FLY; x += 4) {
+            const uint32_t w[16] = {v[x].x,     v[x].y,     v[x].z,     v[x].w,     v[x + 1].x, v[x + 1].y,
+                                    v[x + 1].z, v[x + 1].w, v[x + 2].x, v[x + 2].y, v[x + 2].z, v[x + 2].w,
+                                    v[x + 3].x, v[x + 3].y, v[x + 3].z, v[x + 3].w};
+            tc_st16(tmem + lanes + C::kColQ + (c0 + x) * 4, w);
+          }
         } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int ch = c * 4 + j;
-            *reinterpret_cast<uint4*>(sm + C::kOffQ + (ch >> 3) * 16384 + sw128(row, ch & 7)) = v[j];
-          }
+          for (int j = 0; j < FLY; ++j)
+            *reinterpret_cast<uint4*>(sm + C::kOffQ + ((c0 + j) >> 3) * 16384 + sw128(row, (c0 + j) & 7)) = v[j];
         }
       }
       if constexpr (C::kQTmem) {
@@ -366,7 +369,7 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
     };
-    if (grp == 0) load_q(at);
+    load_q(at);
     int i = 0, item = 0;
     while (i < n && ok && !*abort_flag) {
       // one item, or this CTA's part of it: units i .. last
@@ -385,31 +388,39 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
         const int b = i & 1, pb = PB == 2 ? b : 0, k0 = (at.u + i - begin_i) * 64;
         if (!(ok = warp_wait(&s_full[b], (i >> 1) & 1))) break;
         tc_after();
-        // Two passes over the unit's scores, 32 columns at a time: they stay in tensor memory
-        // between the maximum and the exponentials, which halves the registers and the code.
         const int rem = lim - k0;
-        const bool cut = k0 + 64 > all;   // some row does not see the whole unit
         float mt = -INFINITY;
+        uint32_t r0[32], r1[32];   // the unit's scores
         if (any) {
+          if (k0 + 64 > all) {   // some row does not see the whole unit: -inf in place
 #pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
-            uint32_t r[32];
-            tc_ld32(tmem + lanes + C::kColS + b * 64 + c * 32, r);
-            tc_wait_ld();
-            if (cut) {
+            for (int c = 0; c < 4; ++c) {
+              uint32_t r[16];
+              tc_ld16(tmem + lanes + C::kColS + b * 64 + c * 16, r);
+              tc_wait_ld();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) r[j] = c * 32 + j < rem ? r[j] : 0xFF800000u;
+              for (int j = 0; j < 16; ++j) r[j] = c * 16 + j < rem ? r[j] : 0xFF800000u;
+              tc_st16(tmem + lanes + C::kColS + b * 64 + c * 16, r);
             }
-            float mx[4] = {mt, mt, mt, mt};
-#pragma unroll
-            for (int j = 0; j < 32; j += 8) {
-#pragma unroll
-              for (int x = 0; x < 4; ++x)
-                mx[x] = fmaxf(mx[x], fmaxf(__uint_as_float(r[j + x]), __uint_as_float(r[j + 4 + x])));
-            }
-            mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            tc_wait_st();
           }
-          mt *= sc;
+          tc_ld32(tmem + lanes + C::kColS + b * 64, r0);
+          tc_ld32(tmem + lanes + C::kColS + b * 64 + 32, r1);
+          tc_wait_ld();
+        }
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[b]);
+        if (any) {
+          float mx[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) mx[x] = fmaxf(__uint_as_float(r0[x]), __uint_as_float(r1[x]));
+#pragma unroll
+          for (int j = 4; j < 32; j += 4) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) mx[x] = fmaxf(mx[x], fmaxf(__uint_as_float(r0[j + x]), __uint_as_float(r1[j + x])));
+          }
+          mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
         }
         // the row's reference maximum after the unit before this one
         float m_old = m_ref;
@@ -453,41 +464,30 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
         if (i >= PB && !(ok = warp_wait(&pv_done[(i - PB) & 1], ((i - PB) >> 1) & 1))) break;
         if (any) {
           float sums[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
-            uint32_t r[32];
-            tc_ld32(tmem + lanes + C::kColS + b * 64 + c * 32, r);
-            tc_wait_ld();
-            if (cut) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) r[j] = c * 32 + j < rem ? r[j] : 0xFF800000u;
-            }
+          auto weights = [&](const uint32_t (&r)[32], int c) {
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
               uint32_t w[4];
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 // 2^(scale log2(e) s - m): one fma and one ex2; a masked key's -inf gives 0
-                w[j] = pack2<BF>(ex2_approx(fmaf(__uint_as_float(r[8 * x + 2 * j]), sc, off)),
-                                 ex2_approx(fmaf(__uint_as_float(r[8 * x + 2 * j + 1]), sc, off)));
-                const float2 p = unpack2<BF>(w[j]);   // the rounded weights are summed: see the rows form
-                sums[j] += p.x + p.y;
+                const float p0 = ex2_approx(fmaf(__uint_as_float(r[8 * x + 2 * j]), sc, off));
+                const float p1 = ex2_approx(fmaf(__uint_as_float(r[8 * x + 2 * j + 1]), sc, off));
+                sums[j] += p0 + p1;
+                w[j] = pack2<BF>(p0, p1);
               }
               *reinterpret_cast<uint4*>(sm + C::kOffP + pb * C::kPBytes + sw128(row, c * 4 + x)) =
                   make_uint4(w[0], w[1], w[2], w[3]);
             }
-          }
+          };
+          weights(r0, 0);
+          weights(r1, 1);
           l_run += (sums[0] + sums[1]) + (sums[2] + sums[3]);
         }
         fence_proxy_async_smem();
         tc_before();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&p_full[b]);
-          mbar_arrive(&s_free[b]);
-        }
-        // Q of the next item may follow once every S of this one is made
-        if (i == last && i + 1 < n) load_q(next);
+        if (lane == 0) mbar_arrive(&p_full[b]);
         if (edge) {
           // bad values that the helpers took out of V, for the rows that see them
           if (!(ok = warp_wait(&pv_done[b], (i >> 1) & 1))) break;
@@ -501,6 +501,11 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
         }
       }
       if (!ok) break;
+      // Q of the next item may follow once the last S of this one is made
+      if (last + 1 < n) {
+        if (NG == 2 && (last & 1) != grp && !(ok = warp_wait(&s_full[last & 1], (last >> 1) & 1))) break;
+        load_q(next);
+      }
       // the item's rows, or this part's; two groups take half of the columns each
       if (NG == 2) {
         if ((last & 1) != grp) {
@@ -530,14 +535,18 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
         const float inv = 1.f / l_run;
         const int64_t tok = at.r.q0 + t;
         const int head = at.head * a.group + hl;
+        uint4 gn[4];   // the gate's next 32 dims, in flight
+        auto gate_of = [&](int c) {
+          if (!whole || !a.gate || !valid) return;
+          const uint4* gp = reinterpret_cast<const uint4*>(a.gate + tok * a.g_tok + head * a.g_head + c * 32);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) gn[j] = __ldg(gp + j);
+        };
+        gate_of(grp * (HD / 32 / NG));
 #pragma unroll 1
         for (int c = grp * (HD / 32 / NG); c < (grp + 1) * (HD / 32 / NG); ++c) {
-          uint4 gv[4];
-          if (whole && a.gate && valid) {
-            const uint4* gp = reinterpret_cast<const uint4*>(a.gate + tok * a.g_tok + head * a.g_head + c * 32);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) gv[j] = __ldg(gp + j);
-          }
+          uint4 gv[4] = {gn[0], gn[1], gn[2], gn[3]};
+          if (c + 1 < (grp + 1) * (HD / 32 / NG)) gate_of(c + 1);
           uint32_t r[32];
           tc_ld32(tmem + lanes + C::kColO + c * 32, r);
           tc_wait_ld();
@@ -668,9 +677,25 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
       constexpr int ATOMS = Q8 ? 1 : HD / 64, LR = Q8 ? C::kRaw : RING;
       const int rows = min(a.c.page_size, 64), part = lane / ATOMS, atom = lane % ATOMS;
       const bool mine = part * rows < 64;
-      auto page_of = [&](const Pos& p) -> int {   // -1: outside the pool, read as 0
+        // Page ids come from two windows of 32 table entries, a lane holding one of each: the
+      // second is in flight while the first is used.
+      int w_req = -1, w0 = 0, cur = -1, nxt = -1;
+      auto entry = [&](int b, int i) { return i < a.width ? a.table[b * a.table_ld + i] : -1; };
+      auto page_of = [&](const Pos& p) -> int {   // of this lane's box; -1: outside the pool, read as 0
+        const int first = (p.u * 64) >> a.shift, base = first & ~31;   // (a unit's pages share a window)
+        if (p.b != w_req || base != w0) {
+          if (p.b == w_req && base == w0 + 32) {
+            cur = nxt;
+          } else {
+            cur = entry(p.b, base + lane);
+          }
+          w_req = p.b;
+          w0 = base;
+          nxt = entry(p.b, base + 32 + lane);
+        }
         const int key = p.u * 64 + part * rows;
-        return mine && key < p.r.keys ? a.table[p.b * a.table_ld + (key >> a.shift)] : -1;
+        const int page = __shfl_sync(0xffffffffu, cur, ((mine ? key : p.u * 64) >> a.shift) & 31);
+        return mine && key < p.r.keys ? page : -1;
       };
       int h = 0;
       bool ok = true;
