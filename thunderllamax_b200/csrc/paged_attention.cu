@@ -19,18 +19,19 @@ namespace tlx {
 namespace {
 
 // -------------------------------------------------------------------- combine
-// A block per split item and row (or every gridDim.y-th row).  The pieces' maxima give
-// their weights; groups of threads sum a contiguous share of the pieces each, in piece
-// order, and the groups' sums are added in order, so the result does not depend on when
-// anything ran.
+// Joins the pieces of the split items: the maxima give the pieces' weights, the weighted
+// rows are added in piece order (with many pieces: eight shares in order, then the shares),
+// so the result does not depend on when anything ran.  A warp takes a row of an item of up
+// to kWarpPieces pieces, else a block does, a warp per share: a few pieces cost one trip to
+// memory for their statistics and one for their rows, without a barrier.
+constexpr int kWarpPieces = 16;
+
 template <bool BF, int HD, int ROWS>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constant__ AttnArgs a) {
-  constexpr int kLanes = HD / 4, kGroups = 256 / kLanes;
-  __shared__ float wgt[kMaxPieces];
-  __shared__ float4 acc[256];
-  __shared__ float red[8];
+  constexpr int VEC = HD / 32;   // values of a lane
+  __shared__ float acc[8][HD];
   griddep_wait();
-  const int tid = threadIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (a.by_item) {   // only the items of this launch have written their entry
     const Req r = get_req(a, blockIdx.x / a.c.kv_heads);
     if (r.n < 1 || r.n * static_cast<int64_t>(a.group) > a.rows_limit) return;
@@ -40,74 +41,71 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constan
   const int b = d.z >> 10, head = d.z & 1023;
   const Req r = get_req(a, b);
   const int tt = 128 / a.group, t0 = d.w * tt, rows = min(tt, r.n - t0) * a.group;
-  const int c0 = d.x >> 1, pieces = min(d.y - c0 + 1, kMaxPieces);
+  const int c0 = d.x >> 1, pieces = d.y - c0 + 1;
   auto slot_of = [&](int p) { return p == 0 ? d.x : 2 * (c0 + p); };
-  auto block_reduce = [&](float v, bool is_max) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float w = __shfl_xor_sync(0xffffffffu, v, o);
-      v = is_max ? fmaxf(v, w) : v + w;
-    }
-    __syncthreads();
-    if ((tid & 31) == 0) red[tid >> 5] = v;
-    __syncthreads();
-    v = red[0];
-#pragma unroll
-    for (int w = 1; w < 8; ++w) v = is_max ? fmaxf(v, red[w]) : v + red[w];
-    return v;
-  };
-  const int lane = tid % kLanes, grp = tid / kLanes;
-  const int p0 = pieces * grp / kGroups, p1 = pieces * (grp + 1) / kGroups;
-  for (int row = blockIdx.y; row < rows; row += gridDim.y) {
+  const bool alone = pieces <= kWarpPieces;   // a warp for the row
+  // pieces of this warp
+  const int p0 = alone ? 0 : pieces * warp / 8, p1 = alone ? pieces : pieces * (warp + 1) / 8;
+  for (int row = alone ? blockIdx.y * 8 + warp : blockIdx.y; row < rows; row += gridDim.y * (alone ? 8 : 1)) {
     float m = -INFINITY;
-    for (int p = tid; p < pieces; p += 256) m = fmaxf(m, a.ml[slot_of(p) * ROWS + row].x);
-    m = block_reduce(m, true);   // (its barriers also end the last row's use of wgt and acc)
+    for (int p = lane; p < pieces; p += 32) m = fmaxf(m, a.ml[slot_of(p) * ROWS + row].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float base = m == -INFINITY ? 0.f : m;
     float l = 0.f;
-    for (int p = tid; p < pieces; p += 256) {
+    for (int p = lane; p < pieces; p += 32) {
       const float2 x = a.ml[slot_of(p) * ROWS + row];
-      const float w = ex2_approx(x.x - base);
-      wgt[p] = w;
-      l += x.y * w;
+      l += x.y * ex2_approx(x.x - base);
     }
-    l = block_reduce(l, false);   // (its barriers also publish wgt)
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    float s[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) s[j] = 0.f;
+#pragma unroll 4
     for (int p = p0; p < p1; ++p) {
-      const float4 v =
-          *reinterpret_cast<const float4*>(a.part + (static_cast<int64_t>(slot_of(p)) * ROWS + row) * HD + 4 * lane);
-      const float w = wgt[p];
-      s.x = fmaf(v.x, w, s.x);
-      s.y = fmaf(v.y, w, s.y);
-      s.z = fmaf(v.z, w, s.z);
-      s.w = fmaf(v.w, w, s.w);
-    }
-    acc[tid] = s;
-    __syncthreads();
-    if (grp == 0) {
-      for (int k = 1; k < kGroups; ++k) {
-        const float4 v = acc[k * kLanes + lane];
-        s.x += v.x;
-        s.y += v.y;
-        s.z += v.z;
-        s.w += v.w;
+      const int slot = slot_of(p);
+      const float w = ex2_approx(a.ml[slot * ROWS + row].x - base);
+      const float2* v = reinterpret_cast<const float2*>(a.part + (static_cast<int64_t>(slot) * ROWS + row) * HD) + lane;
+#pragma unroll
+      for (int j = 0; j < VEC; j += 2) {   // dims 64 (j / 2) + 2 lane, + 1
+        const float2 y = v[j * 16];
+        s[j] = fmaf(y.x, w, s[j]);
+        s[j + 1] = fmaf(y.y, w, s[j + 1]);
       }
+    }
+    if (!alone) {
+#pragma unroll
+      for (int j = 0; j < VEC; j += 2) *reinterpret_cast<float2*>(&acc[warp][j * 32 + 2 * lane]) = make_float2(s[j], s[j + 1]);
+      __syncthreads();
+      if (warp == 0) {
+        for (int w = 1; w < 8; ++w) {
+#pragma unroll
+          for (int j = 0; j < VEC; j += 2) {
+            s[j] += acc[w][j * 32 + 2 * lane];
+            s[j + 1] += acc[w][j * 32 + 2 * lane + 1];
+          }
+        }
+      }
+    }
+    if (alone || warp == 0) {
       const int t = t0 + row / a.group, hq = head * a.group + row % a.group;
       const bool sees = min(r.keys, r.kv - r.n_all + t + 1) > 0;
-      float v[4] = {s.x / l, s.y / l, s.z / l, s.w / l};
       const int64_t tok = r.q0 + t;
-      if (a.gate) {
-        const uint2 x = *reinterpret_cast<const uint2*>(a.gate + tok * a.g_tok + hq * a.g_head + 4 * lane);
-        const float2 x0 = unpack2<BF>(x.x), x1 = unpack2<BF>(x.y);
-        v[0] /= 1.f + __expf(-x0.x);
-        v[1] /= 1.f + __expf(-x0.y);
-        v[2] /= 1.f + __expf(-x1.x);
-        v[3] /= 1.f + __expf(-x1.y);
+      const float inv = 1.f / l;
+#pragma unroll
+      for (int j = 0; j < VEC; j += 2) {
+        const int dim = j * 32 + 2 * lane;
+        float v0 = sees ? s[j] * inv : 0.f, v1 = sees ? s[j + 1] * inv : 0.f;
+        if (a.gate) {
+          const float2 x = unpack2<BF>(*reinterpret_cast<const uint32_t*>(a.gate + tok * a.g_tok + hq * a.g_head + dim));
+          v0 = gated(v0, x.x);
+          v1 = gated(v1, x.y);
+        }
+        *reinterpret_cast<uint32_t*>(a.out + tok * a.o_tok + hq * a.o_head + dim) = pack2<BF>(v0, v1);
       }
-      if (!sees) v[0] = v[1] = v[2] = v[3] = 0.f;
-      *reinterpret_cast<uint2*>(a.out + tok * a.o_tok + hq * a.o_head + 4 * lane) =
-          make_uint2(pack2<BF>(v[0], v[1]), pack2<BF>(v[2], v[3]));
     }
+    if (!alone) __syncthreads();   // acc is free for the next row
   }
 }
 

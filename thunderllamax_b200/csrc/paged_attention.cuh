@@ -9,7 +9,6 @@ namespace tlx {
 
 constexpr size_t kPagedErrBytes = 256;   // the workspace starts with the device error word
 constexpr int kRowsMax = 16;             // query rows per KV head of the rows form
-constexpr int kMaxPieces = 1024;         // CTAs of a launch at most
 
 struct AttnArgs {
   tlx_paged_kv c;

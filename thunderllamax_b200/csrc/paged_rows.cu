@@ -432,8 +432,10 @@ int launch_rows(AttnArgs a, void* ws, int sms, cudaStream_t s) {
   using C = RowsCfg<CT, HD>;
   static bool configured = false;
   if (!configured) {
-    if (cudaFuncSetAttribute(paged_rows_kernel<CT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) !=
-        cudaSuccess)
+    // the shared memory of all the CTAs an SM is to hold, not of one
+    if (cudaFuncSetAttribute(paged_rows_kernel<CT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess ||
+        cudaFuncSetAttribute(paged_rows_kernel<CT, HD>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) !=
+            cudaSuccess)
       return TLX_ERR_LAUNCH;
     configured = true;
   }

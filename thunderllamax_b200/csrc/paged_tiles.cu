@@ -18,14 +18,15 @@ namespace {
 //                so one group's exponentials run beside the other's loads and waits, and
 //                hand on the row's reference maximum.  O is rescaled (in tensor memory) only
 //                when a row's maximum grows by more than 2^8, which keeps P in range.
-//   QK warp, PV warp     one thread each issues its MMAs: two issuers, because the waits and
-//                commits of one would leave the tensor pipe idle
-//   loader warp          the K and V halves of the units: one TMA box per page (and 64 dims),
-//                so pages may lie anywhere and what is outside the pool reads as 0
-//   helper warps         16-bit caches: on the PV thread's request take out of V what must
-//                not reach the product (rows past the last key, and infinite or NaN values
-//                where some rows do not see the unit whole); int8 caches: turn every half
-//                into fp16(code * scale)
+//   QK warps, PV warp    one thread each issues its MMAs: several issuers (two for S, the
+//                units in turn), because the waits and commits of one would leave the tensor
+//                pipe idle.  The PV warp also takes out of a 16-bit V what must not reach the
+//                product (rows past the last key, and infinite or NaN values where some rows
+//                do not see the unit whole).
+//   loader warps         the K and V halves of the units: one TMA box per page (and 64 dims),
+//                so pages may lie anywhere and what is outside the pool reads as 0; issuing a
+//                box costs its warp about 100 cycles, so the warps share the boxes of a half
+//   converter warps      (int8 caches) turn every half into fp16(code * scale)
 // Every wait is bounded: a timeout raises the error word, all roles leave, issued MMAs
 // and copies are drained and tensor memory is freed.
 //
@@ -66,16 +67,16 @@ struct TilesCfg {
   static constexpr int kGroups = HD == 256 || kQ8 ? 2 : 1;
   static constexpr int kCtas = kGroups == 2 ? 1 : 2;
   static constexpr int kPBufs = HD == 128 && !kQ8 ? 1 : 2;
-  // 16-bit halves of K or V that the MMAs read, and (int8) halves as they lie in the cache
+  // 16-bit halves that the MMAs read, one half of the ring for K and one for V (so that each
+  // issuer waits for its slots in order), and (int8) halves as they lie in the cache
   static constexpr int kRing = kQ8 && HD == 256 ? 4 : HD == 128 && !kQ8 ? 4 : 6;
   static constexpr int kRaw = !kQ8 ? 0 : HD == 256 ? 3 : 6;
   static constexpr int kRawHalf = kKeys * HD;                   // codes; the scales follow
   static constexpr int kRawBytes = kRawHalf + kKeys * (HD / 16);
   static constexpr int kThreads = kGroups == 2 ? 512 : 256;
-  static constexpr int kQkWarp = 4 * kGroups, kPvWarp = kQkWarp + 1, kLoadWarp = kQkWarp + 2, kHelpWarp = kQkWarp + 3;
-  // int8: the four warps of the last warpgroup, a fixed share of the chunks each
-  static constexpr int kHelpFirst = kQ8 ? kThreads / 32 - 4 : kHelpWarp;
-  static constexpr int kHelpers = kThreads / 32 - kHelpFirst;
+  static constexpr int kQkWarp = 4 * kGroups, kPvWarp = kQkWarp + kGroups, kLoadWarp = kPvWarp + 1;
+  static constexpr int kLoaders = kQ8 ? 1 : kGroups == 2 ? 4 : 2;
+  static constexpr int kConvWarp = kThreads / 32 - 4;           // int8: four converters
   // registers after the roles part (of the 128 of the launch)
   static constexpr int kRegsSoftmax = kGroups == 2 ? 168 : 184;
   static constexpr int kRegsOther = kGroups == 2 ? 88 : 72;
@@ -146,7 +147,7 @@ __device__ __forceinline__ int64_t units_before(const AttnArgs& a, const Req& r,
   return s;
 }
 
-// The helpers replace infinite and NaN values of V by 0 in the units that some rows do
+// Infinite and NaN values of V are replaced by 0 in shared memory in the units that some rows do
 // not see whole (0 * inf in the product would reach those rows); this adds weight * value
 // of such keys to the rows that do see them.  Called by whole warps with O at rest; the
 // weights are the rounded ones of the product, from P in shared memory.
@@ -191,40 +192,35 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
   using C = TilesCfg<CT, HD>;
   constexpr bool BF = CT == CT_BF16, Q8 = C::kQ8;
   static_assert(C::kColO + HD + (C::kQTmem ? C::kColQ - 384 + HD / 2 : 0) <= C::kTmem, "tensor memory");
-  constexpr int NH = C::kHelpers, RING = C::kRing, PB = C::kPBufs, NG = C::kGroups;
+  constexpr int RING = C::kRing, RH = RING / 2, PB = C::kPBufs, NG = C::kGroups;
   extern __shared__ __align__(1024) uint8_t sm[];
   uint64_t* bar = reinterpret_cast<uint64_t*>(sm + C::kOffBar);
-  uint64_t* landed = bar;               // [RING or RAW] TMA -> MMA or helpers
-  uint64_t* raw_free = landed + 6;      // [RAW] helpers -> loader
-  uint64_t* full = raw_free + 6;        // [RING] helpers -> MMA
-  uint64_t* empty = full + 6;           // [RING] MMA -> loader or helpers
+  uint64_t* landed = bar;               // [RING or RAW] TMA -> MMA or converters
+  uint64_t* raw_free = landed + 6;      // [RAW] converters -> loader
+  uint64_t* full = raw_free + 6;        // [RING] converters -> MMA
+  uint64_t* empty = full + 6;           // [RING] MMA -> loaders or converters
   uint64_t* s_full = empty + 6;         // [2] QK -> softmax
   uint64_t* s_free = s_full + 2;        // [2] softmax -> QK
   uint64_t* p_full = s_free + 2;        // [2] softmax -> PV
   uint64_t* pv_done = p_full + 2;       // [2] PV -> softmax
   uint64_t* q_full = pv_done + 2;       // softmax -> QK: Q of the next item is in
   uint64_t* o_free = q_full + 1;        // softmax -> PV: O of the last item is read
-  uint64_t* fix_req = o_free + 1;       // PV -> helpers: a V half to clean
-  uint64_t* fix_done = fix_req + 1;     // helpers -> PV
-  uint64_t* done = fix_done + 1;
-  uint64_t* m_full = done + 1;          // [4][2] between the groups' warps of the same rows: maximum of unit i
+  uint64_t* done = o_free + 1;
+  uint64_t* turn = done + 1;            // [2] QK warp -> QK warp: S of unit i is issued
+  uint64_t* m_full = turn + 2;          // [4][2] between the groups' warps of the same rows: maximum of unit i
   uint64_t* l_full = m_full + 8;        // [4] the same: both groups' sums of an item
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(l_full + 4);
   volatile uint32_t* abort_flag = tmem_holder + 1;
-  // [8] by unit: unit + 1 if the helpers took a bad value out of its V (they are fewer than
-  // 8 units ahead of the softmax)
+  // [8] by unit: unit + 1 if a bad value was taken out of its V (V is fewer than 8 units ahead
+  // of the softmax)
   volatile int* bad = reinterpret_cast<int*>(tmem_holder + 2);
   struct First {
     int tile, head, u;
   };
   First* first_at = reinterpret_cast<First*>(tmem_holder + 10);
-  struct Fix {
-    int slot, valid, edge, unit;   // ring slot (-1: no more), keys of the unit that exist
-  };
-  Fix* fix = reinterpret_cast<Fix*>(tmem_holder + 14);
   volatile float* m_sh = reinterpret_cast<float*>(sm + C::kOffX);   // [128]
   volatile float* l_sh = m_sh + 128;                                 // [2 items][2 groups][128]
-  static_assert((4 * 6 + 25) * 8 + 14 * 4 + sizeof(Fix) <= 512 && RING <= 6 && C::kRaw <= 6, "barrier area");
+  static_assert((4 * 6 + 25) * 8 + 13 * 4 <= 512 && RING <= 6 && C::kRaw <= 6, "barrier area");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   griddep_launch_dependents();
@@ -260,9 +256,9 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
   }
   if (tid == 0) {
     for (int i = 0; i < 6; ++i) {
-      mbar_init(&landed[i], Q8 ? 33 : 1);   // int8: 32 lanes' copies of the scales as well
-      mbar_init(&raw_free[i], NH);
-      mbar_init(&full[i], NH);
+      mbar_init(&landed[i], Q8 ? 33 : C::kLoaders);   // int8: 32 lanes' copies of the scales as well
+      mbar_init(&raw_free[i], 4);
+      mbar_init(&full[i], 4);
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 8; ++i) bad[i] = 0;
@@ -274,9 +270,8 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
     }
     mbar_init(q_full, 4 * NG);
     mbar_init(o_free, 4 * NG);
-    mbar_init(fix_req, 1);
-    mbar_init(fix_done, NH);
-    mbar_init(done, 2);
+    mbar_init(done, NG + 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&turn[i], 1);
     for (int i = 0; i < 8; ++i) mbar_init(&m_full[i], 1);
     for (int i = 0; i < 4; ++i) mbar_init(&l_full[i], 2);
     *abort_flag = 0u;
@@ -489,7 +484,7 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[b]);
         if (edge) {
-          // bad values that the helpers took out of V, for the rows that see them
+          // bad values that were taken out of V, for the rows that see them
           if (!(ok = warp_wait(&pv_done[b], (i >> 1) & 1))) break;
           tc_after();
           if (bad[i & 7] == i + 1)
@@ -588,34 +583,42 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
     if (!ok) fail();
   } else {
     reg_dec<C::kRegsOther>();
-    if (warp == C::kQkWarp) {
+    if (warp < C::kPvWarp) {
       // --------------------------------------------------------------- S = Q K^T
       if (lane == 0) {
         bool ok = true;
         int left = min(at.of - at.u, n), item = 0;
         bool starts = true;
         for (int i = 0; i < n && ok && !*abort_flag; ++i) {
-          // K(i) follows i Ks and the Vs before V(i - 1), which it precedes unless it starts an item
-          const int h = 2 * i - (starts ? 0 : 1), slot = h % RING, b = i & 1;
-          if (starts && !(ok = tc_wait(q_full, item & 1))) break;
-          if (!(ok = tc_wait(Q8 ? &full[slot] : &landed[slot], (h / RING) & 1))) break;
-          if (!(ok = tc_wait(&s_free[b], ((i >> 1) & 1) ^ 1))) break;
-          tc_after();
-          const uint64_t kd = sw128_desc(sbase + slot * C::kHalf);
-          const uint64_t qd = C::kQTmem ? 0ull : sw128_desc(sbase + C::kOffQ);
+          const int slot = i % RH, b = i & 1;
+          if (NG == 1 || b == warp - C::kQkWarp) {   // (two warps: the units in turn)
+            if (!(ok = tc_wait(&s_free[b], ((i >> 1) & 1) ^ 1))) break;
+            if (!(ok = tc_wait(Q8 ? &full[slot] : &landed[slot], (i / RH) & 1))) break;
+            // the turn first: it says that Q of the item before has come, so that the wait for this
+            // item's Q is for the next phase
+            if (NG == 2 && i > 0 && !(ok = tc_wait(&turn[b ^ 1], ((i - 1) >> 1) & 1))) break;
+            if (starts && !(ok = tc_wait(q_full, item & 1))) break;
+            tc_after();
+            const uint64_t kd = sw128_desc(sbase + slot * C::kHalf);
+            const uint64_t qd = C::kQTmem ? 0ull : sw128_desc(sbase + C::kOffQ);
 #pragma unroll 1
-          for (int x = 0; x < HD / 64; ++x) {   // (a loop over the atoms: see the note on code size)
+            for (int x = 0; x < HD / 64; ++x) {   // (a loop over the atoms: see the note on code size)
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const uint64_t bd = kd + (x * 8192 + y * 32) / 16;   // the address field, in 16-byte units
-              if constexpr (C::kQTmem)
-                tc_mma_ts(tmem + C::kColS + b * 64, tmem + C::kColQ + x * 32 + y * 8, bd, C::kIdescQK, x + y > 0 ? 1u : 0u);
-              else
-                tc_mma(tmem + C::kColS + b * 64, qd + (x * 16384 + y * 32) / 16, bd, C::kIdescQK, x + y > 0 ? 1u : 0u);
+              for (int y = 0; y < 4; ++y) {
+                const uint64_t bd = kd + (x * 8192 + y * 32) / 16;   // the address field, in 16-byte units
+                if constexpr (C::kQTmem)
+                  tc_mma_ts(tmem + C::kColS + b * 64, tmem + C::kColQ + x * 32 + y * 8, bd, C::kIdescQK, x + y > 0 ? 1u : 0u);
+                else
+                  tc_mma(tmem + C::kColS + b * 64, qd + (x * 16384 + y * 32) / 16, bd, C::kIdescQK, x + y > 0 ? 1u : 0u);
+              }
             }
+            if (NG == 2) {
+              tc_before();
+              mbar_arrive(&turn[b]);
+            }
+            tc_commit(&s_full[b]);
+            tc_commit(&empty[slot]);
           }
-          tc_commit(&s_full[b]);
-          tc_commit(&empty[slot]);
           starts = --left == 0;
           if (starts && i + 1 < n) {
             next_item(at);
@@ -629,22 +632,38 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
       }
     } else if (warp == C::kPvWarp) {
       // ---------------------------------------------------------------- O += P V
-      if (lane == 0) {
-        bool ok = true;
-        int left = min(at.of - at.u, n), item = 0, fixes = 0, all = seen_by_all(at);
-        bool starts = true;
-        for (int i = 0; i < n && ok && !*abort_flag; ++i) {
-          // V(i) follows i Vs and i + 1 Ks, and K(i + 1) unless unit i ends an item
-          const int h = 2 * i + 1 + (left != 1 && i + 1 < n ? 1 : 0), slot = h % RING, pb = PB == 2 ? i & 1 : 0;
-          if (starts && item > 0 && !(ok = tc_wait(o_free, (item - 1) & 1))) break;
-          if (!(ok = tc_wait(Q8 ? &full[slot] : &landed[slot], (h / RING) & 1))) break;
-          if (!Q8 && at.u * 64 + 64 > all) {
-            *fix = Fix{slot, at.r.keys - at.u * 64, all < min(at.u * 64 + 64, at.r.keys), i};
-            mbar_arrive(fix_req);
-            if (!(ok = tc_wait(fix_done, fixes++ & 1))) break;
+      bool ok = true;
+      int left = min(at.of - at.u, n), item = 0, all = seen_by_all(at);
+      bool starts = true;
+      for (int i = 0; i < n && ok && !*abort_flag; ++i) {
+        const int slot = RH + i % RH, pb = PB == 2 ? i & 1 : 0;
+        if (starts && item > 0 && !(ok = warp_wait(o_free, (item - 1) & 1))) break;
+        if (!(ok = warp_wait(Q8 ? &full[slot] : &landed[slot], (i / RH) & 1))) break;
+        if (!Q8 && at.u * 64 + 64 > all) {   // not seen whole by some row, or with fewer than 64 keys
+          const int valid = at.r.keys - at.u * 64;
+          const bool edge = all < min(at.u * 64 + 64, at.r.keys);
+          uint8_t* hb = sm + slot * C::kHalf;
+          bool any_bad = false;
+          for (int idx = (edge ? 0 : valid * (HD / 8)) + lane; idx < 64 * HD / 8; idx += 32) {
+            const int key = idx / (HD / 8), ch = idx % (HD / 8);
+            uint4* p = reinterpret_cast<uint4*>(hb + (ch >> 3) * 8192 + sw128(key, ch & 7));
+            if (key >= valid) {
+              *p = make_uint4(0u, 0u, 0u, 0u);
+            } else {
+              const uint4 x = *p;
+              uint32_t w[4] = {x.x, x.y, x.z, x.w};
+              if (drop_bad<BF>(w[0]) | drop_bad<BF>(w[1]) | drop_bad<BF>(w[2]) | drop_bad<BF>(w[3])) {
+                *p = make_uint4(w[0], w[1], w[2], w[3]);
+                any_bad = true;
+              }
+            }
           }
-          if (!(ok = tc_wait(&p_full[i & 1], (i >> 1) & 1))) break;
-          tc_after();
+          if (any_bad) bad[i & 7] = i + 1;
+          fence_proxy_async_smem();
+        }
+        if (!(ok = warp_wait(&p_full[i & 1], (i >> 1) & 1))) break;
+        tc_after();
+        if (lane == 0) {
           const uint64_t pd = sw128_desc(sbase + C::kOffP + pb * C::kPBytes);
           const uint64_t vd = sw128_desc_mn(sbase + slot * C::kHalf, 8192);
 #pragma unroll
@@ -652,32 +671,33 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
             tc_mma(tmem + C::kColO, pd + k * 2, vd + k * 128, C::kIdescPV, (!starts || k > 0) ? 1u : 0u);
           tc_commit(&pv_done[i & 1]);
           tc_commit(&empty[slot]);
-          ++at.u;
-          starts = --left == 0;
-          if (starts && i + 1 < n) {
-            next_item(at);
-            left = at.of;
-            all = seen_by_all(at);
-            ++item;
-          }
         }
-        if (!ok) fail();
-        if constexpr (!Q8) {
-          fix->slot = -1;
-          mbar_arrive(fix_req);
+        __syncwarp();
+        ++at.u;
+        starts = --left == 0;
+        if (starts && i + 1 < n) {
+          next_item(at);
+          left = at.of;
+          all = seen_by_all(at);
+          ++item;
         }
+      }
+      if (!ok) fail();
+      if (lane == 0) {
         tc_commit(done);
         if (!tc_wait(done, 0)) fail();
       }
-    } else if (warp == C::kLoadWarp) {
+    } else if (warp < C::kLoadWarp + C::kLoaders) {
       // ------------------------------------------------------------------ loader
       // Halves in MMA order: per unit K(i) then V(i - 1), or V(i - 1) first where unit i
       // starts an item.  A lane owns one TMA box of a half: 64 dims (int8: all) of the keys
       // of one page.
-      constexpr int ATOMS = Q8 ? 1 : HD / 64, LR = Q8 ? C::kRaw : RING;
-      const int rows = min(a.c.page_size, 64), part = lane / ATOMS, atom = lane % ATOMS;
+      constexpr int ATOMS = Q8 ? 1 : HD / 64, LR = Q8 ? C::kRaw : RING, NL = C::kLoaders;
+      const int rows = min(a.c.page_size, 64), box = lane * NL + warp - C::kLoadWarp, part = box / ATOMS, atom = box % ATOMS;
       const bool mine = part * rows < 64;
-        // Page ids come from two windows of 32 table entries, a lane holding one of each: the
+      // bytes of this warp's boxes
+      const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine)) * rows * (Q8 ? HD : 128);
+      // Page ids come from two windows of 32 table entries, a lane holding one of each: the
       // second is in flight while the first is used.
       int w_req = -1, w0 = 0, cur = -1, nxt = -1;
       auto entry = [&](int b, int i) { return i < a.width ? a.table[b * a.table_ld + i] : -1; };
@@ -699,11 +719,11 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
       };
       int h = 0;
       bool ok = true;
-      auto load = [&](bool v, const auto& x) {
+      auto load = [&](bool v, int unit, const auto& x) {
         const int page = x.page, u = x.u, head = x.head, keys = x.keys;
-        const int slot = h % LR;
-        if (!(ok = warp_wait(Q8 ? &raw_free[slot] : &empty[slot], ((h / LR) & 1) ^ 1))) return;
-        if (lane == 0) mbar_arrive_expect_tx(&landed[slot], Q8 ? C::kRawHalf : C::kHalf);
+        const int slot = Q8 ? h % LR : (v ? RH : 0) + unit % RH, turn_of = Q8 ? h / LR : unit / RH;
+        if (!(ok = warp_wait(Q8 ? &raw_free[slot] : &empty[slot], (turn_of & 1) ^ 1))) return;
+        if (lane == 0) mbar_arrive_expect_tx(&landed[slot], bytes);
         __syncwarp();
         const int in = (u * 64 + part * rows) & (a.c.page_size - 1);
         uint8_t* dst = Q8 ? sm + C::kOffRaw + slot * C::kRawBytes + part * rows * HD
@@ -735,7 +755,7 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
       bool starts = true;
       while (v < n && ok && !*abort_flag) {
         const bool is_v = i - v == 2 || (i - v == 1 && (starts || i == n));
-        load(is_v, is_v ? (i - v == 2 ? v2 : v1) : k);
+        load(is_v, is_v ? v : i, is_v ? (i - v == 2 ? v2 : v1) : k);
         if (is_v) {
           ++v;
           continue;
@@ -757,62 +777,41 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
       if (!ok) fail();
       if (!ok || *abort_flag) {   // no copy may still be in flight when the CTA ends
         if constexpr (Q8) cp_async_wait_all();
-        for (int f = max(0, h - LR); f < h; ++f) tc_wait(&landed[f % LR], (f / LR) & 1);
-      }
-    } else if (warp >= C::kHelpFirst) {
-      // ----------------------------------------------------------------- helpers
-      const int hw = warp - C::kHelpFirst;
-      bool ok = true;
-      if constexpr (!Q8) {
-        for (int k = 0; ok && !*abort_flag; ++k) {
-          if (!(ok = warp_wait(fix_req, k & 1))) break;
-          const Fix f = *fix;
-          if (f.slot < 0) break;
-          uint8_t* hb = sm + f.slot * C::kHalf;
-          bool any_bad = false;
-          for (int idx = hw * 32 + lane; idx < 64 * HD / 8; idx += NH * 32) {
-            const int key = idx / (HD / 8), ch = idx % (HD / 8);
-            uint4* p = reinterpret_cast<uint4*>(hb + (ch >> 3) * 8192 + sw128(key, ch & 7));
-            if (key >= f.valid) {
-              *p = make_uint4(0u, 0u, 0u, 0u);
-            } else if (f.edge) {
-              const uint4 x = *p;
-              uint32_t w[4] = {x.x, x.y, x.z, x.w};
-              if (drop_bad<BF>(w[0]) | drop_bad<BF>(w[1]) | drop_bad<BF>(w[2]) | drop_bad<BF>(w[3])) {
-                *p = make_uint4(w[0], w[1], w[2], w[3]);
-                any_bad = true;
-              }
-            }
-          }
-          if (any_bad) bad[f.unit & 7] = f.unit + 1;
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(fix_done);
+        if constexpr (Q8) {
+          for (int f = max(0, h - LR); f < h; ++f) tc_wait(&landed[f % LR], (f / LR) & 1);
+        } else {
+          for (int f = max(0, i - RH); f < i; ++f) tc_wait(&landed[f % RH], (f / RH) & 1);
+          for (int f = max(0, v - RH); f < v; ++f) tc_wait(&landed[RH + f % RH], (f / RH) & 1);
         }
-      } else {
+      }
+    } else if (Q8 && warp >= C::kConvWarp) {
+      // -------------------------------------------------------------- converters
+      const int hw = warp - C::kConvWarp;
+      bool ok = true;
+      if constexpr (Q8) {
         constexpr int CPK = HD / 16;   // 16-byte chunks of a cached row
         int h = 0;
-        auto convert = [&](int valid, bool edge, int unit) {
-          const int slot = h % RING, rs = h % C::kRaw;
-          if (!(ok = warp_wait(&landed[rs], (h / C::kRaw) & 1)) || !(ok = warp_wait(&empty[slot], ((h / RING) & 1) ^ 1))) return;
+        auto convert = [&](bool v, int unit, int valid, bool edge) {
+          const int slot = (v ? RH : 0) + unit % RH, rs = h % C::kRaw;
+          if (!(ok = warp_wait(&landed[rs], (h / C::kRaw) & 1)) || !(ok = warp_wait(&empty[slot], ((unit / RH) & 1) ^ 1))) return;
           const uint8_t* raw = sm + C::kOffRaw + rs * C::kRawBytes;
           bool any_bad = false;
-          constexpr int PER = 64 * CPK / (NH * 32), BATCH = PER > 2 ? 2 : PER;
-          static_assert(PER * NH * 32 == 64 * CPK, "the helpers' shares");
+          constexpr int PER = 64 * CPK / (128), BATCH = PER > 2 ? 2 : PER;
+          static_assert(PER * 128 == 64 * CPK, "the converters' shares");
   #pragma unroll 1
           for (int x0 = 0; x0 < PER; x0 += BATCH) {
             uint4 x[BATCH];
             uint32_t sc[BATCH];
   #pragma unroll
             for (int x1 = 0; x1 < BATCH; ++x1) {   // 16 dims: 16-bit chunks 2 ch and 2 ch + 1
-              const int idx = (x0 + x1) * NH * 32 + hw * 32 + lane, key = idx / CPK, ch = idx % CPK;
+              const int idx = (x0 + x1) * 128 + hw * 32 + lane, key = idx / CPK, ch = idx % CPK;
               x[x1] = *reinterpret_cast<const uint4*>(raw + idx * 16);
               sc[x1] = *reinterpret_cast<const uint16_t*>(raw + C::kRawHalf + key * (HD / 16) + (ch >> 1) * 2);
               if (key >= valid) sc[x1] = 0u;   // rows past the last key: +-0
             }
   #pragma unroll
             for (int x1 = 0; x1 < BATCH; ++x1) {
-              const int idx = (x0 + x1) * NH * 32 + hw * 32 + lane, key = idx / CPK, ch = idx % CPK;
+              const int idx = (x0 + x1) * 128 + hw * 32 + lane, key = idx / CPK, ch = idx % CPK;
               const uint32_t s2 = sc[x1] | sc[x1] << 16;
               const uint32_t in[4] = {x[x1].x, x[x1].y, x[x1].z, x[x1].w};
               uint32_t o[8];
@@ -854,7 +853,7 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
         while (v < n && ok && !*abort_flag) {
           const bool is_v = i - v == 2 || (i - v == 1 && (starts || i == n));
           const Half x = is_v ? (i - v == 2 ? v2 : v1) : k;
-          convert(x.valid, is_v && x.edge, v);
+          convert(is_v, is_v ? v : i, x.valid, is_v && x.edge);
           if (is_v) {
             ++v;
             continue;
@@ -922,8 +921,10 @@ int launch_tiles(AttnArgs a, void* ws, int sms, cudaStream_t s) {
   using C = TilesCfg<CT, HD>;
   static bool configured = false;
   if (!configured) {
-    if (cudaFuncSetAttribute(paged_tiles_kernel<CT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) !=
-        cudaSuccess)
+    // the shared memory of all the CTAs an SM is to hold, not of one
+    if (cudaFuncSetAttribute(paged_tiles_kernel<CT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess ||
+        cudaFuncSetAttribute(paged_tiles_kernel<CT, HD>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) !=
+            cudaSuccess)
       return TLX_ERR_LAUNCH;
     configured = true;
   }
@@ -934,7 +935,7 @@ int launch_tiles(AttnArgs a, void* ws, int sms, cudaStream_t s) {
   if (!page_map(&km, a.c, a.c.k, a.c.k_stride) || !page_map(&vm, a.c, a.c.v, a.c.v_stride)) return TLX_ERR_LAUNCH;
   paged_tiles_kernel<CT, HD><<<ctas, C::kThreads, C::kSmem, s>>>(a, km, vm, static_cast<uint32_t*>(ws));
   if (cudaGetLastError() != cudaSuccess) return TLX_ERR_LAUNCH;
-  return launch_combine(a, CT == CT_BF16, 128, ctas, 16, s);
+  return launch_combine(a, CT == CT_BF16, 128, ctas, 32, s);
 }
 
 }  // namespace
