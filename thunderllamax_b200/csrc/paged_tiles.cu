@@ -48,8 +48,18 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(b))
       : "memory");
 }
+// A bounded wait: the first poll in place, the others out of line (one copy for all).
+__device__ __forceinline__ bool wait_on(uint64_t* b, uint32_t parity) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < kMbarPollLimit; ++i)
+    if (mbar_try_wait(b, parity)) return true;
+  return false;
+}
+__device__ __forceinline__ bool thread_wait(uint64_t* b, uint32_t parity) {
+  return mbar_try_wait(b, parity) || wait_on(b, parity);
+}
 __device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t parity) {
-  const bool ok = tc_wait(b, parity);
+  const bool ok = thread_wait(b, parity);
   __syncwarp();   // what follows is for the whole warp
   return ok;
 }
@@ -97,7 +107,7 @@ struct TilesCfg {
 };
 
 // sum over i < n of floor((a i + b) / m): the Euclid-like recursion, as a loop
-__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+__device__ __noinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
   int64_t s = 0;
   while (n > 0) {
     if (a >= m) {
@@ -134,7 +144,7 @@ __device__ __forceinline__ int tile_units(const AttnArgs& a, const Req& r, int t
   return max(1, (tile_keys(a, r, tile) + 63) >> 6);
 }
 // units of one KV head in the tiles before `tile`
-__device__ __forceinline__ int64_t units_before(const AttnArgs& a, const Req& r, int tile) {
+__device__ __noinline__ int64_t units_before(const AttnArgs& a, const Req& r, int tile) {
   const int64_t tt = tile_tokens(a), c = static_cast<int64_t>(r.kv) - r.n_all;
   const int full = min(tile, r.n / static_cast<int>(tt));   // tiles with all their tokens
   int64_t s = 0;
@@ -183,6 +193,28 @@ __device__ __noinline__ void restore_bad_values(const AttnArgs& a, int b, int he
     tc_st32(o_tmem + c * 32, r);
     tc_wait_st();
   }
+}
+
+// An item (tile of a request's rows, KV head) and a unit of it.
+struct Pos {
+  int b, tile, head, u, of, tiles;
+  Req r;
+};
+__device__ __forceinline__ Pos item_after(const AttnArgs& a, Pos p) {
+  p.u = 0;
+  if (++p.head == a.c.kv_heads) {
+    p.head = 0;
+    if (++p.tile == p.tiles) {
+      p.tile = 0;
+      do {
+        if (++p.b >= a.n_req) return p;
+        p.r = get_req(a, p.b);
+        p.tiles = tile_count(a, p.r);
+      } while (p.tiles == 0);
+    }
+    p.of = tile_units(a, p.r, p.tile);
+  }
+  return p;
 }
 
 template <int CT, int HD>
@@ -287,10 +319,6 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
     *abort_flag = 1u;
   };
 
-  struct Pos {
-    int b, tile, head, u, of, tiles;
-    Req r;
-  };
   Pos at;
   at.b = st.b;
   at.r = get_req(a, st.b);
@@ -300,21 +328,7 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
   at.u = first_at->u;
   at.of = tile_units(a, at.r, at.tile);
   // the next item (not called past the last unit of the launch)
-  auto next_item = [&](Pos& p) {
-    p.u = 0;
-    if (++p.head == a.c.kv_heads) {
-      p.head = 0;
-      if (++p.tile == p.tiles) {
-        p.tile = 0;
-        do {
-          if (++p.b >= a.n_req) return;
-          p.r = get_req(a, p.b);
-          p.tiles = tile_count(a, p.r);
-        } while (p.tiles == 0);
-      }
-      p.of = tile_units(a, p.r, p.tile);
-    }
-  };
+  auto next_item = [&](Pos& p) { p = item_after(a, p); };
 
   // keys that every row of the item's tile sees; a unit past them needs care (is not seen
   // whole by some row, or holds fewer than 64 keys)
@@ -592,12 +606,12 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
         for (int i = 0; i < n && ok && !*abort_flag; ++i) {
           const int slot = i % RH, b = i & 1;
           if (NG == 1 || b == warp - C::kQkWarp) {   // (two warps: the units in turn)
-            if (!(ok = tc_wait(&s_free[b], ((i >> 1) & 1) ^ 1))) break;
-            if (!(ok = tc_wait(Q8 ? &full[slot] : &landed[slot], (i / RH) & 1))) break;
+            if (!(ok = thread_wait(&s_free[b], ((i >> 1) & 1) ^ 1))) break;
+            if (!(ok = thread_wait(Q8 ? &full[slot] : &landed[slot], (i / RH) & 1))) break;
             // the turn first: it says that Q of the item before has come, so that the wait for this
             // item's Q is for the next phase
-            if (NG == 2 && i > 0 && !(ok = tc_wait(&turn[b ^ 1], ((i - 1) >> 1) & 1))) break;
-            if (starts && !(ok = tc_wait(q_full, item & 1))) break;
+            if (NG == 2 && i > 0 && !(ok = thread_wait(&turn[b ^ 1], ((i - 1) >> 1) & 1))) break;
+            if (starts && !(ok = thread_wait(q_full, item & 1))) break;
             tc_after();
             const uint64_t kd = sw128_desc(sbase + slot * C::kHalf);
             const uint64_t qd = C::kQTmem ? 0ull : sw128_desc(sbase + C::kOffQ);
@@ -628,7 +642,7 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
         }
         if (!ok) fail();
         tc_commit(done);   // every issued MMA has completed before tensor memory is released
-        if (!tc_wait(done, 0)) fail();
+        if (!thread_wait(done, 0)) fail();
       }
     } else if (warp == C::kPvWarp) {
       // ---------------------------------------------------------------- O += P V
@@ -685,7 +699,7 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
       if (!ok) fail();
       if (lane == 0) {
         tc_commit(done);
-        if (!tc_wait(done, 0)) fail();
+        if (!thread_wait(done, 0)) fail();
       }
     } else if (warp < C::kLoadWarp + C::kLoaders) {
       // ------------------------------------------------------------------ loader
@@ -778,10 +792,10 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
       if (!ok || *abort_flag) {   // no copy may still be in flight when the CTA ends
         if constexpr (Q8) cp_async_wait_all();
         if constexpr (Q8) {
-          for (int f = max(0, h - LR); f < h; ++f) tc_wait(&landed[f % LR], (f / LR) & 1);
+          for (int f = max(0, h - LR); f < h; ++f) thread_wait(&landed[f % LR], (f / LR) & 1);
         } else {
-          for (int f = max(0, i - RH); f < i; ++f) tc_wait(&landed[f % RH], (f / RH) & 1);
-          for (int f = max(0, v - RH); f < v; ++f) tc_wait(&landed[RH + f % RH], (f / RH) & 1);
+          for (int f = max(0, i - RH); f < i; ++f) thread_wait(&landed[f % RH], (f / RH) & 1);
+          for (int f = max(0, v - RH); f < v; ++f) thread_wait(&landed[RH + f % RH], (f / RH) & 1);
         }
       }
     } else if (Q8 && warp >= C::kConvWarp) {
