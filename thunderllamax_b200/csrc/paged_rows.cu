@@ -265,81 +265,100 @@ __global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel
     __syncthreads();   // P is in
     // O of this warp's dims
     const uint8_t* vb = kb + kOffV;
-    // a key that some rows do not see must not reach them through 0 * inf or 0 * NaN
-    const bool edge = at.r.n > 1 && (at.u + 1) * KT > at.r.kv - at.r.n_all;
-    auto product = [&](int j, const uint32_t (&pf)[4], uint32_t v0, uint32_t v1, int k16) {
-      if (edge && __any_sync(0xffffffffu, bad16<BF>(v0) || bad16<BF>(v1))) {
-        const int key = at.u * KT + k16 * 16 + 2 * q;
-        for (int t = 0; t < at.r.n; ++t) {   // each token's rows with the keys it sees
-          const int lim = at.r.kv - at.r.n_all + t + 1;
-          const uint32_t w0 = v0 & ((key < lim ? 0xFFFFu : 0u) | (key + 1 < lim ? 0xFFFF0000u : 0u));
-          const uint32_t w1 = v1 & ((key + 8 < lim ? 0xFFFFu : 0u) | (key + 9 < lim ? 0xFFFF0000u : 0u));
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
-          mma16<BF>(d, pf, w0, w1);
-          if (g / a.group == t) {
-            o[j][0] += d[0];
-            o[j][1] += d[1];
-          }
-          if ((g + 8) / a.group == t) {
-            o[j][2] += d[2];
-            o[j][3] += d[3];
+    // A key that some rows do not see must not reach them through 0 * inf or 0 * NaN: units
+    // with such keys are looked over first (of single tokens there are none).
+    bool slow = false;
+    if (at.r.n > 1 && (at.u + 1) * KT > at.r.kv - at.r.n_all + 1) {
+      bool found = false;
+      for (int key = max(0, at.r.kv - at.r.n_all + 1 - at.u * KT) + warp; key < KT; key += 4) {
+        if constexpr (Q8) {   // (any product may overflow where the scale passes 65504 / 128)
+          for (int x = lane; x < HD / 32; x += 32)
+            found |= !(fabsf(__half2float(*reinterpret_cast<const __half*>(kb + kOffVs + key * C::kScaleRow + 2 * x))) < 511.f);
+        } else {
+          for (int x = lane; x < CPR; x += 32) {
+            const uint4 v = lds128(vb + key * C::kRow + x * 16);
+            found |= bad16<BF>(v.x) || bad16<BF>(v.y) || bad16<BF>(v.z) || bad16<BF>(v.w);
           }
         }
-      } else {
-        mma16<BF>(o[j], pf, v0, v1);
+      }
+      slow = __syncthreads_or(found);
+    }
+    auto product = [&](int j, const uint32_t (&pf)[4], uint32_t v0, uint32_t v1, int) { mma16<BF>(o[j], pf, v0, v1); };
+    // the same token by token, each with the keys it sees
+    auto careful = [&](int j, const uint32_t (&pf)[4], uint32_t v0, uint32_t v1, int k16) {
+      const int key = at.u * KT + k16 * 16 + 2 * q;
+#pragma unroll 1
+      for (int t = 0; t < at.r.n; ++t) {
+        const int lim = at.r.kv - at.r.n_all + t + 1;
+        const uint32_t w0 = v0 & ((key < lim ? 0xFFFFu : 0u) | (key + 1 < lim ? 0xFFFF0000u : 0u));
+        const uint32_t w1 = v1 & ((key + 8 < lim ? 0xFFFFu : 0u) | (key + 9 < lim ? 0xFFFF0000u : 0u));
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
+        mma16<BF>(d, pf, w0, w1);
+        if (g / a.group == t) {
+          o[j][0] += d[0];
+          o[j][1] += d[1];
+        }
+        if ((g + 8) / a.group == t) {
+          o[j][2] += d[2];
+          o[j][3] += d[3];
+        }
       }
     };
+    auto unit_product = [&](auto&& product) {
+#pragma unroll 1
+      for (int k = 0; k < KT / 16; ++k) {
+        uint32_t pf[4];
+        ldsm4(pf, pbase + ((lane & 7) + ((lane >> 3) & 1) * 8) * C::kPPitch + (2 * k + (lane >> 4)) * 16);
+        if constexpr (Q8) {
+          // lane (g, q): keys 2q, 2q+1, 2q+8, 2q+9 and DB contiguous dims from DB g on
+          uint32_t w[4][DB > 4 ? 2 : 1];
+          uint32_t sh[4];
 #pragma unroll
-    for (int k = 0; k < KT / 16; ++k) {
-      uint32_t pf[4];
-      ldsm4(pf, pbase + ((lane & 7) + ((lane >> 3) & 1) * 8) * C::kPPitch + (2 * k + (lane >> 4)) * 16);
-      if constexpr (Q8) {
-        // lane (g, q): keys 2q, 2q+1, 2q+8, 2q+9 and DB contiguous dims from DB g on
-        uint32_t w[4][DB > 4 ? 2 : 1];
-        uint32_t sh[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int row = k * 16 + 2 * q + (e & 1) + (e >> 1) * 8;
-          const int byte = warp * DW + DB * g;
-          const int ch = HD == 64 ? (byte >> 4) ^ ((row >> 1) & 3) : (byte >> 4) ^ (((row >> 1) & 3) << 1);
-          const uint8_t* p = vb + row * C::kRow + ch * 16 + (byte & 15);
-          if constexpr (DB == 8) {
-            const uint2 v = lds64(p);
-            w[e][0] = v.x;
-            w[e][1] = v.y;
-          } else if constexpr (DB == 4) {
-            w[e][0] = lds32(p);
-          } else {
-            w[e][0] = *reinterpret_cast<const uint16_t*>(p);
+          for (int e = 0; e < 4; ++e) {
+            const int row = k * 16 + 2 * q + (e & 1) + (e >> 1) * 8;
+            const int byte = warp * DW + DB * g;
+            const int ch = HD == 64 ? (byte >> 4) ^ ((row >> 1) & 3) : (byte >> 4) ^ (((row >> 1) & 3) << 1);
+            const uint8_t* p = vb + row * C::kRow + ch * 16 + (byte & 15);
+            if constexpr (DB == 8) {
+              const uint2 v = lds64(p);
+              w[e][0] = v.x;
+              w[e][1] = v.y;
+            } else if constexpr (DB == 4) {
+              w[e][0] = lds32(p);
+            } else {
+              w[e][0] = *reinterpret_cast<const uint16_t*>(p);
+            }
+            sh[e] = *reinterpret_cast<const uint16_t*>(kb + kOffVs + row * C::kScaleRow + (byte >> 5) * 2);
           }
-          sh[e] = *reinterpret_cast<const uint16_t*>(kb + kOffVs + row * C::kScaleRow + (byte >> 5) * 2);
-        }
-        const uint32_t s01 = prmt(sh[0], sh[1], 0x5410u), s23 = prmt(sh[2], sh[3], 0x5410u);
+          const uint32_t s01 = prmt(sh[0], sh[1], 0x5410u), s23 = prmt(sh[2], sh[3], 0x5410u);
 #pragma unroll
-        for (int h = 0; h < (DB > 4 ? 2 : 1); ++h) {
-          // (key 2q, key 2q+1) byte pairs of four dims
-          const uint32_t a01 = prmt(w[0][h], w[1][h], 0x5140u), a23 = prmt(w[0][h], w[1][h], 0x7362u);
-          const uint32_t c01 = prmt(w[2][h], w[3][h], 0x5140u), c23 = prmt(w[2][h], w[3][h], 0x7362u);
-          const int j = 4 * h;
-          product(j, pf, dq2(a01, 0x5140u, s01), dq2(c01, 0x5140u, s23), k);
-          product(j + 1, pf, dq2(a01, 0x7362u, s01), dq2(c01, 0x7362u, s23), k);
-          if constexpr (DB >= 4) {
-            product(j + 2, pf, dq2(a23, 0x5140u, s01), dq2(c23, 0x5140u, s23), k);
-            product(j + 3, pf, dq2(a23, 0x7362u, s01), dq2(c23, 0x7362u, s23), k);
+          for (int h = 0; h < (DB > 4 ? 2 : 1); ++h) {
+            // (key 2q, key 2q+1) byte pairs of four dims
+            const uint32_t a01 = prmt(w[0][h], w[1][h], 0x5140u), a23 = prmt(w[0][h], w[1][h], 0x7362u);
+            const uint32_t c01 = prmt(w[2][h], w[3][h], 0x5140u), c23 = prmt(w[2][h], w[3][h], 0x7362u);
+            const int j = 4 * h;
+            product(j, pf, dq2(a01, 0x5140u, s01), dq2(c01, 0x5140u, s23), k);
+            product(j + 1, pf, dq2(a01, 0x7362u, s01), dq2(c01, 0x7362u, s23), k);
+            if constexpr (DB >= 4) {
+              product(j + 2, pf, dq2(a23, 0x5140u, s01), dq2(c23, 0x5140u, s23), k);
+              product(j + 3, pf, dq2(a23, 0x7362u, s01), dq2(c23, 0x7362u, s23), k);
+            }
           }
-        }
-      } else {
+        } else {
 #pragma unroll
-        for (int j = 0; j < DB; j += 2) {
-          const int row = k * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
-          const int ch = (warp * DB + j + (lane >> 4)) ^ (row & 7);
-          uint32_t v[4];
-          ldsm4t(v, smem_u32(vb) + row * C::kRow + ch * 16);
-          product(j, pf, v[0], v[1], k);
-          product(j + 1, pf, v[2], v[3], k);
+          for (int j = 0; j < DB; j += 2) {
+            const int row = k * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+            const int ch = (warp * DB + j + (lane >> 4)) ^ (row & 7);
+            uint32_t v[4];
+            ldsm4t(v, smem_u32(vb) + row * C::kRow + ch * 16);
+            product(j, pf, v[0], v[1], k);
+            product(j + 1, pf, v[2], v[3], k);
+          }
         }
       }
-    }
+    };
+    if (slow) unit_product(careful);
+    else unit_product(product);
     // the end of the item, or of this CTA's part of it
     if (at.u + 1 == at.of || i + 1 == n_units) {
       first = true;

@@ -48,15 +48,12 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(b))
       : "memory");
 }
-// A bounded wait: the first poll in place, the others out of line (one copy for all).
-__device__ __forceinline__ bool wait_on(uint64_t* b, uint32_t parity) {
+// A bounded wait, as little code as it can be.
+__device__ __forceinline__ bool thread_wait(uint64_t* b, uint32_t parity) {
 #pragma unroll 1
   for (uint32_t i = 0; i < kMbarPollLimit; ++i)
     if (mbar_try_wait(b, parity)) return true;
   return false;
-}
-__device__ __forceinline__ bool thread_wait(uint64_t* b, uint32_t parity) {
-  return mbar_try_wait(b, parity) || wait_on(b, parity);
 }
 __device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t parity) {
   const bool ok = thread_wait(b, parity);
@@ -378,29 +375,122 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
     };
-    load_q(at);
-    int i = 0, item = 0;
-    while (i < n && ok && !*abort_flag) {
-      // one item, or this CTA's part of it: units i .. last
-      const int count = min(at.of - at.u, n - i), begin_i = i, last = i + count - 1;
+    int i = 0, item = -1, last = -1, begin_i = 0;
+    Pos next = at;
+    float m_ref, l_run;
+    for (;;) {
+      // (one site each for the Q load, the item's units and its end: see the note on code size)
+      const bool more = i < n;
+      if (more) {   // Q of the next item may follow once the last S of this one is made
+        if (NG == 2 && item >= 0 && (last & 1) != grp && !(ok = warp_wait(&s_full[last & 1], (last >> 1) & 1))) break;
+        load_q(next);
+      }
       const int t = at.tile * tt + t_in;
       const bool valid = t_in < tt && t < at.r.n;
       const int lim = valid ? max(0, min(at.r.keys, at.r.kv - at.r.n_all + t + 1)) : 0;   // keys < lim
-      const int all = seen_by_all(at);
       const bool any = __any_sync(0xffffffffu, valid);   // a warp without rows only keeps the barriers going
+      if (item >= 0) {
+        // the item's rows, or this part's; two groups take half of the columns each
+        if (NG == 2) {
+          if ((last & 1) != grp) {
+            if (!(ok = warp_wait(&m_full[qd * 2 + (last & 1)], (last >> 1) & 1))) break;
+            const float m_end = m_sh[row];
+            if (m_ref != m_end) {
+              l_run *= ex2_approx(m_ref - m_end);
+              m_ref = m_end;
+            }
+          }
+          volatile float* l2 = l_sh + (item & 1) * 256;
+          l2[grp * 128 + row] = l_run;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&l_full[qd]);
+          if (!(ok = warp_wait(&l_full[qd], item & 1))) break;
+          l_run = l2[row] + l2[128 + row];
+        }
+        if (!(ok = warp_wait(&pv_done[last & 1], (last >> 1) & 1))) break;
+        tc_after();
+        const int64_t begin = st.u0 + begin_i - at.u, end = begin + at.of;   // the item's units
+        const bool whole = begin >= st.u0 && end <= st.u1;
+        const int slot = 2 * blockIdx.x + (begin > st.u0 ? 1 : 0);
+        if (tid == 0 && begin >= st.u0 && !whole)
+          a.desc[blockIdx.x] = make_int4(slot, range_of(st.units, end - 1, st.ctas), at.b << 10 | at.head, at.tile);
+        if (any) {
+          const bool sees = lim > 0;
+          const float inv = 1.f / l_run;
+          const int64_t tok = at.r.q0 + t;
+          const int head = at.head * a.group + hl;
+          uint4 gn[4];   // the gate's next 32 dims, in flight
+          auto gate_of = [&](int c) {
+            if (!whole || !a.gate || !valid) return;
+            const uint4* gp = reinterpret_cast<const uint4*>(a.gate + tok * a.g_tok + head * a.g_head + c * 32);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) gn[j] = __ldg(gp + j);
+          };
+          gate_of(grp * (HD / 32 / NG));
+#pragma unroll 1
+          for (int c = grp * (HD / 32 / NG); c < (grp + 1) * (HD / 32 / NG); ++c) {
+            uint4 gv[4] = {gn[0], gn[1], gn[2], gn[3]};
+            if (c + 1 < (grp + 1) * (HD / 32 / NG)) gate_of(c + 1);
+            uint32_t r[32];
+            tc_ld32(tmem + lanes + C::kColO + c * 32, r);
+            tc_wait_ld();
+            if (!valid) continue;
+            if (!whole) {
+              float4* dst = reinterpret_cast<float4*>(a.part + (static_cast<int64_t>(slot) * 128 + row) * HD + c * 32);
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                dst[j] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
+                                     __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
+            } else {
+              uint4* dst = reinterpret_cast<uint4*>(a.out + tok * a.o_tok + head * a.o_head + c * 32);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                float v[8];
+#pragma unroll
+                for (int x = 0; x < 8; ++x) v[x] = sees ? __uint_as_float(r[8 * j + x]) * inv : 0.f;
+                if (a.gate) {
+                  const uint32_t gw[4] = {gv[j].x, gv[j].y, gv[j].z, gv[j].w};
+#pragma unroll
+                  for (int x = 0; x < 4; ++x) {
+                    const float2 y = unpack2<BF>(gw[x]);
+                    v[2 * x] = gated(v[2 * x], y.x);
+                    v[2 * x + 1] = gated(v[2 * x + 1], y.y);
+                  }
+                }
+                dst[j] = make_uint4(pack2<BF>(v[0], v[1]), pack2<BF>(v[2], v[3]), pack2<BF>(v[4], v[5]), pack2<BF>(v[6], v[7]));
+              }
+            }
+          }
+          if (!whole && valid && grp == 0) a.ml[slot * 128 + row] = make_float2(m_ref, l_run);
+        }
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(o_free);
+      }
+      if (!more || *abort_flag) break;
+      at = next;
+      ++item;
+      // one item, or this CTA's part of it: units i .. last
+      begin_i = i;
+      last = i + min(at.of - at.u, n - i) - 1;
+      const int tn = at.tile * tt + t_in;
+      const bool here = t_in < tt && tn < at.r.n;
+      const int lim_n = here ? max(0, min(at.r.keys, at.r.kv - at.r.n_all + tn + 1)) : 0;   // keys < lim_n
+      const int all = seen_by_all(at);
+      const bool run = __any_sync(0xffffffffu, here);
       // m_ref: the row's reference maximum as this group last knew it, its sum relative to it
-      float m_ref = -INFINITY, l_run = 0.f;
-      Pos next = at;
+      m_ref = -INFINITY;
+      l_run = 0.f;
       if (last + 1 < n) next_item(next);
       for (; i <= last && ok; ++i) {
         if (NG == 2 && (i & 1) != grp) continue;
         const int b = i & 1, pb = PB == 2 ? b : 0, k0 = (at.u + i - begin_i) * 64;
         if (!(ok = warp_wait(&s_full[b], (i >> 1) & 1))) break;
         tc_after();
-        const int rem = lim - k0;
+        const int rem = lim_n - k0;
         float mt = -INFINITY;
         uint32_t r0[32], r1[32];   // the unit's scores
-        if (any) {
+        if (run) {
           if (k0 + 64 > all) {   // some row does not see the whole unit: -inf in place
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
@@ -420,7 +510,7 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
         tc_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_free[b]);
-        if (any) {
+        if (run) {
           float mx[4];
 #pragma unroll
           for (int x = 0; x < 4; ++x) mx[x] = fmaxf(__uint_as_float(r0[x]), __uint_as_float(r1[x]));
@@ -446,18 +536,18 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
             if (!(ok = warp_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1))) break;   // O is at rest
             tc_after();
 #pragma unroll 1
-            for (int c = 0; c < HD / 32; ++c) {
-              uint32_t r[32];
-              tc_ld32(tmem + lanes + C::kColO + c * 32, r);
+            for (int c = 0; c < HD / 16; ++c) {
+              uint32_t r[16];
+              tc_ld16(tmem + lanes + C::kColO + c * 16, r);
               tc_wait_ld();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * cor);
-              tc_st32(tmem + lanes + C::kColO + c * 32, r);
+              for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * cor);
+              tc_st16(tmem + lanes + C::kColO + c * 16, r);
             }
             tc_wait_st();
           }
         }
-        const bool edge = any && all < min(k0 + 64, at.r.keys);   // some row does not see the unit whole
+        const bool edge = run && all < min(k0 + 64, at.r.keys);   // some row does not see the unit whole
         if (NG == 2) {
           m_sh[row] = m_new;
           tc_before();
@@ -471,7 +561,7 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
         const float off = m_ref == -INFINITY ? 0.f : -m_ref;
         // the P buffer is free once the product that read it is done
         if (i >= PB && !(ok = warp_wait(&pv_done[(i - PB) & 1], ((i - PB) >> 1) & 1))) break;
-        if (any) {
+        if (run) {
           float sums[4] = {0.f, 0.f, 0.f, 0.f};
           auto weights = [&](const uint32_t (&r)[32], int c) {
 #pragma unroll
@@ -502,7 +592,7 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
           if (!(ok = warp_wait(&pv_done[b], (i >> 1) & 1))) break;
           tc_after();
           if (bad[i & 7] == i + 1)
-            restore_bad_values<CT, HD>(a, at.b, at.head, k0, at.r.keys, lim, sm + C::kOffP + pb * C::kPBytes, row,
+            restore_bad_values<CT, HD>(a, at.b, at.head, k0, at.r.keys, lim_n, sm + C::kOffP + pb * C::kPBytes, row,
                                        tmem + lanes + C::kColO);
           tc_before();
           __syncwarp();
@@ -510,89 +600,6 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
         }
       }
       if (!ok) break;
-      // Q of the next item may follow once the last S of this one is made
-      if (last + 1 < n) {
-        if (NG == 2 && (last & 1) != grp && !(ok = warp_wait(&s_full[last & 1], (last >> 1) & 1))) break;
-        load_q(next);
-      }
-      // the item's rows, or this part's; two groups take half of the columns each
-      if (NG == 2) {
-        if ((last & 1) != grp) {
-          if (!(ok = warp_wait(&m_full[qd * 2 + (last & 1)], (last >> 1) & 1))) break;
-          const float m_end = m_sh[row];
-          if (m_ref != m_end) {
-            l_run *= ex2_approx(m_ref - m_end);
-            m_ref = m_end;
-          }
-        }
-        volatile float* l2 = l_sh + (item & 1) * 256;
-        l2[grp * 128 + row] = l_run;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&l_full[qd]);
-        if (!(ok = warp_wait(&l_full[qd], item & 1))) break;
-        l_run = l2[row] + l2[128 + row];
-      }
-      if (!(ok = warp_wait(&pv_done[last & 1], (last >> 1) & 1))) break;
-      tc_after();
-      const int64_t begin = st.u0 + begin_i - at.u, end = begin + at.of;   // the item's units
-      const bool whole = begin >= st.u0 && end <= st.u1;
-      const int slot = 2 * blockIdx.x + (begin > st.u0 ? 1 : 0);
-      if (tid == 0 && begin >= st.u0 && !whole)
-        a.desc[blockIdx.x] = make_int4(slot, range_of(st.units, end - 1, st.ctas), at.b << 10 | at.head, at.tile);
-      if (any) {
-        const bool sees = lim > 0;
-        const float inv = 1.f / l_run;
-        const int64_t tok = at.r.q0 + t;
-        const int head = at.head * a.group + hl;
-        uint4 gn[4];   // the gate's next 32 dims, in flight
-        auto gate_of = [&](int c) {
-          if (!whole || !a.gate || !valid) return;
-          const uint4* gp = reinterpret_cast<const uint4*>(a.gate + tok * a.g_tok + head * a.g_head + c * 32);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) gn[j] = __ldg(gp + j);
-        };
-        gate_of(grp * (HD / 32 / NG));
-#pragma unroll 1
-        for (int c = grp * (HD / 32 / NG); c < (grp + 1) * (HD / 32 / NG); ++c) {
-          uint4 gv[4] = {gn[0], gn[1], gn[2], gn[3]};
-          if (c + 1 < (grp + 1) * (HD / 32 / NG)) gate_of(c + 1);
-          uint32_t r[32];
-          tc_ld32(tmem + lanes + C::kColO + c * 32, r);
-          tc_wait_ld();
-          if (!valid) continue;
-          if (!whole) {
-            float4* dst = reinterpret_cast<float4*>(a.part + (static_cast<int64_t>(slot) * 128 + row) * HD + c * 32);
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              dst[j] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
-                                   __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
-          } else {
-            uint4* dst = reinterpret_cast<uint4*>(a.out + tok * a.o_tok + head * a.o_head + c * 32);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              float v[8];
-#pragma unroll
-              for (int x = 0; x < 8; ++x) v[x] = sees ? __uint_as_float(r[8 * j + x]) * inv : 0.f;
-              if (a.gate) {
-                const uint32_t gw[4] = {gv[j].x, gv[j].y, gv[j].z, gv[j].w};
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                  const float2 y = unpack2<BF>(gw[x]);
-                  v[2 * x] = gated(v[2 * x], y.x);
-                  v[2 * x + 1] = gated(v[2 * x + 1], y.y);
-                }
-              }
-              dst[j] = make_uint4(pack2<BF>(v[0], v[1]), pack2<BF>(v[2], v[3]), pack2<BF>(v[4], v[5]), pack2<BF>(v[6], v[7]));
-            }
-          }
-        }
-        if (!whole && valid && grp == 0) a.ml[slot * 128 + row] = make_float2(m_ref, l_run);
-      }
-      tc_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(o_free);
-      at = next;
-      ++item;
     }
     if (!ok) fail();
   } else {
@@ -654,22 +661,22 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
         if (starts && item > 0 && !(ok = warp_wait(o_free, (item - 1) & 1))) break;
         if (!(ok = warp_wait(Q8 ? &full[slot] : &landed[slot], (i / RH) & 1))) break;
         if (!Q8 && at.u * 64 + 64 > all) {   // not seen whole by some row, or with fewer than 64 keys
-          const int valid = at.r.keys - at.u * 64;
-          const bool edge = all < min(at.u * 64 + 64, at.r.keys);
-          uint8_t* hb = sm + slot * C::kHalf;
+          // from the first key that some row does not see; a lane owns one chunk of every row
+          // (of every second or fourth row)
+          constexpr int CH = HD / 8, STEP = 32 / CH;
+          const int valid = at.r.keys - at.u * 64, from = max(0, all - at.u * 64), ch = lane % CH;
+          uint8_t* hc = sm + slot * C::kHalf + (ch >> 3) * 8192;
           bool any_bad = false;
-          for (int idx = (edge ? 0 : valid * (HD / 8)) + lane; idx < 64 * HD / 8; idx += 32) {
-            const int key = idx / (HD / 8), ch = idx % (HD / 8);
-            uint4* p = reinterpret_cast<uint4*>(hb + (ch >> 3) * 8192 + sw128(key, ch & 7));
+#pragma unroll 2
+          for (int key = from / STEP * STEP + lane / CH; key < 64; key += STEP) {
+            uint4* p = reinterpret_cast<uint4*>(hc + sw128(key, ch & 7));
+            const uint4 x = *p;
+            uint32_t w[4] = {x.x, x.y, x.z, x.w};
             if (key >= valid) {
               *p = make_uint4(0u, 0u, 0u, 0u);
-            } else {
-              const uint4 x = *p;
-              uint32_t w[4] = {x.x, x.y, x.z, x.w};
-              if (drop_bad<BF>(w[0]) | drop_bad<BF>(w[1]) | drop_bad<BF>(w[2]) | drop_bad<BF>(w[3])) {
-                *p = make_uint4(w[0], w[1], w[2], w[3]);
-                any_bad = true;
-              }
+            } else if ((drop_bad<BF>(w[0]) | drop_bad<BF>(w[1]) | drop_bad<BF>(w[2]) | drop_bad<BF>(w[3])) && key >= from) {
+              *p = make_uint4(w[0], w[1], w[2], w[3]);
+              any_bad = true;
             }
           }
           if (any_bad) bad[i & 7] = i + 1;
