@@ -26,20 +26,31 @@ namespace {
 // memory for their statistics and one for their rows, without a barrier.
 constexpr int kWarpPieces = 16;
 
-template <bool BF, int HD, int ROWS>
-__global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constant__ AttnArgs a) {
+struct CombineArgs {
+  AttnArgs a;
+  SplitSet set[2];   // rows form, tiles form
+};
+
+template <bool BF, int HD>
+__global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constant__ CombineArgs ca) {
   constexpr int VEC = HD / 32;   // values of a lane
   __shared__ float acc[8][HD];
   griddep_wait();
+  const AttnArgs& a = ca.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (a.by_item) {   // only the items of this launch have written their entry
-    const Req r = get_req(a, blockIdx.x / a.c.kv_heads);
-    if (r.n < 1 || r.n * static_cast<int64_t>(a.group) > a.rows_limit) return;
+  const bool second = static_cast<int>(blockIdx.x) >= ca.set[0].items;
+  const SplitSet& set = ca.set[second ? 1 : 0];
+  const int index = blockIdx.x - (second ? ca.set[0].items : 0), slots = set.row_slots;
+  const int4 d = set.desc[index];   // {slot of the first piece, last CTA, request << 10 | KV head, tile}
+  int b = index / a.c.kv_heads;
+  if (!set.by_item) {
+    if (d.x < 0) return;
+    b = d.z >> 10;
   }
-  const int4 d = a.desc[blockIdx.x];   // {slot of the first piece, last CTA, request << 10 | KV head, tile}
-  if (d.x < 0) return;
-  const int b = d.z >> 10, head = d.z & 1023;
   const Req r = get_req(a, b);
+  // (an entry by item is this launch's only if the request has units in this form)
+  if (set.by_item && (r.n < 1 || r.n * static_cast<int64_t>(a.group) > a.rows_limit || d.x < 0)) return;
+  const int head = d.z & 1023;
   const int tt = 128 / a.group, t0 = d.w * tt, rows = min(tt, r.n - t0) * a.group;
   const int c0 = d.x >> 1, pieces = d.y - c0 + 1;
   auto slot_of = [&](int p) { return p == 0 ? d.x : 2 * (c0 + p); };
@@ -47,14 +58,19 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constan
   // pieces of this warp
   const int p0 = alone ? 0 : pieces * warp / 8, p1 = alone ? pieces : pieces * (warp + 1) / 8;
   for (int row = alone ? blockIdx.y * 8 + warp : blockIdx.y; row < rows; row += gridDim.y * (alone ? 8 : 1)) {
-    float m = -INFINITY;
-    for (int p = lane; p < pieces; p += 32) m = fmaxf(m, a.ml[slot_of(p) * ROWS + row].x);
+    // statistics of the first 64 pieces stay with their lane
+    const float2 none = make_float2(-INFINITY, 0.f);
+    const float2 x0 = lane < pieces ? set.ml[slot_of(lane) * slots + row] : none;
+    const float2 x1 = 32 + lane < pieces ? set.ml[slot_of(32 + lane) * slots + row] : none;
+    float m = fmaxf(x0.x, x1.x);
+    for (int p = 64 + lane; p < pieces; p += 32) m = fmaxf(m, set.ml[slot_of(p) * slots + row].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    for (int p = lane; p < pieces; p += 32) {
-      const float2 x = a.ml[slot_of(p) * ROWS + row];
+    const float w0 = ex2_approx(x0.x - base), w1 = ex2_approx(x1.x - base);
+    float l = x0.y * w0 + x1.y * w1;
+    for (int p = 64 + lane; p < pieces; p += 32) {
+      const float2 x = set.ml[slot_of(p) * slots + row];
       l += x.y * ex2_approx(x.x - base);
     }
 #pragma unroll
@@ -65,8 +81,9 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constan
 #pragma unroll 4
     for (int p = p0; p < p1; ++p) {
       const int slot = slot_of(p);
-      const float w = ex2_approx(a.ml[slot * ROWS + row].x - base);
-      const float2* v = reinterpret_cast<const float2*>(a.part + (static_cast<int64_t>(slot) * ROWS + row) * HD) + lane;
+      float w = __shfl_sync(0xffffffffu, p < 32 ? w0 : w1, p & 31);
+      if (p >= 64) w = ex2_approx(set.ml[slot * slots + row].x - base);
+      const float2* v = reinterpret_cast<const float2*>(set.part + (static_cast<int64_t>(slot) * slots + row) * HD) + lane;
 #pragma unroll
       for (int j = 0; j < VEC; j += 2) {   // dims 64 (j / 2) + 2 lane, + 1
         const float2 y = v[j * 16];
@@ -79,6 +96,7 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constan
       for (int j = 0; j < VEC; j += 2) *reinterpret_cast<float2*>(&acc[warp][j * 32 + 2 * lane]) = make_float2(s[j], s[j + 1]);
       __syncthreads();
       if (warp == 0) {
+#pragma unroll 1
         for (int w = 1; w < 8; ++w) {
 #pragma unroll
           for (int j = 0; j < VEC; j += 2) {
@@ -116,38 +134,34 @@ int sm_count() {
   return n > 0 ? n : 148;
 }
 
-int launch_dependent(const void* kern, dim3 grid, dim3 block, cudaStream_t stream, void** args) {
+template <bool BF>
+const void* combine_kernel(int hd) {
+  return hd == 256   ? reinterpret_cast<const void*>(paged_combine_kernel<BF, 256>)
+         : hd == 128 ? reinterpret_cast<const void*>(paged_combine_kernel<BF, 128>)
+                     : reinterpret_cast<const void*>(paged_combine_kernel<BF, 64>);
+}
+
+int launch_combine(CombineArgs& ca, bool bf, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
+  // rows of an item: one a block (many pieces), or eight; the tiles form's blocks walk theirs
+  cfg.gridDim = dim3(ca.set[0].items + ca.set[1].items, std::max(ca.set[0].rows, std::min(32, ca.set[1].rows)));
+  cfg.blockDim = dim3(256);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelExC(&cfg, kern, args) == cudaSuccess ? TLX_OK : TLX_ERR_LAUNCH;
-}
-
-template <bool BF, int HD>
-const void* combine_kernel(int row_slots) {
-  return row_slots == kRowsMax ? reinterpret_cast<const void*>(paged_combine_kernel<BF, HD, kRowsMax>)
-                               : reinterpret_cast<const void*>(paged_combine_kernel<BF, HD, 128>);
+  void* args[] = {&ca};
+  return cudaLaunchKernelExC(&cfg, bf ? combine_kernel<true>(ca.a.c.head_dim) : combine_kernel<false>(ca.a.c.head_dim),
+                             args) == cudaSuccess
+             ? TLX_OK
+             : TLX_ERR_LAUNCH;
 }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace
-
-int launch_combine(const AttnArgs& a, bool bf, int row_slots, int items, int rows, cudaStream_t stream) {
-  const int hd = a.c.head_dim;
-  const void* kern = bf ? (hd == 256 ? combine_kernel<true, 256>(row_slots) : hd == 128 ? combine_kernel<true, 128>(row_slots) : combine_kernel<true, 64>(row_slots))
-                        : (hd == 256 ? combine_kernel<false, 256>(row_slots) : hd == 128 ? combine_kernel<false, 128>(row_slots) : combine_kernel<false, 64>(row_slots));
-  AttnArgs copy = a;
-  void* args[] = {&copy};
-  return launch_dependent(kern, dim3(items, rows), dim3(256), stream, args);
-}
-
 }  // namespace tlx
 
 using namespace tlx;
@@ -159,7 +173,7 @@ size_t tlx_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim
       (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return 0;
   const int sms = sm_count();
-  return std::max(paged_rows_bytes(head_dim, sms), paged_tiles_bytes(head_dim, sms));
+  return kPagedErrBytes + paged_rows_bytes(head_dim, sms) + paged_tiles_bytes(head_dim, sms);
 }
 
 int tlx_paged_attention(const tlx_paged_kv* cache, const int32_t* block_table, int64_t table_stride, int table_width,
@@ -210,12 +224,21 @@ int tlx_paged_attention(const tlx_paged_kv* cache, const int32_t* block_table, i
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   // the requests' lengths are on the device, so each form picks its own requests there
   const int ct = cache_type(cache), sms = sm_count();
-  if (a.group <= kRowsMax) {
-    const int rows_rc = launch_paged_rows(a, ct, ws, sms, s);
-    if (rows_rc) return rows_rc;
+  uint8_t* area = static_cast<uint8_t*>(ws) + kPagedErrBytes;
+  CombineArgs ca;
+  ca.a = a;
+  ca.set[0] = ca.set[1] = SplitSet{nullptr, nullptr, nullptr, 0, 0, 0, 0};
+  const bool rows = a.group <= kRowsMax, tiles = static_cast<int64_t>(a.max_new) * a.group > kRowsMax;
+  if (rows) {
+    const int rc_rows = launch_paged_rows(a, ct, area, sms, s, &ca.set[0]);
+    if (rc_rows) return rc_rows;
   }
-  if (static_cast<int64_t>(a.max_new) * a.group <= kRowsMax) return TLX_OK;
-  return launch_paged_tiles(a, ct, ws, sms, s);
+  if (tiles) {
+    const int rc_tiles = launch_paged_tiles(a, ct, area + paged_rows_bytes(cache->head_dim, sms), static_cast<uint32_t*>(ws),
+                                            sms, rows, s, &ca.set[1]);
+    if (rc_tiles) return rc_tiles;
+  }
+  return launch_combine(ca, ct == CT_BF16, s);
 }
 
 }  // extern "C"

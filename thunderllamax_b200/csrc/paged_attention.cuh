@@ -205,30 +205,38 @@ __device__ __forceinline__ bool drop_bad(uint32_t& w) {
 }
 
 // ---------------------------------------------------------------- host side
+// Each form launches its kernel and says what it may have split: `items` descriptors in its
+// area of the workspace, at most `rows` query rows of an item (row_slots in the buffers).
+struct SplitSet {
+  float* part;
+  float2* ml;
+  int4* desc;
+  int by_item, row_slots, items, rows;
+};
 // split-item area: descriptors, (max, sum) and partial rows of `ctas` CTAs
 struct Split {
-  size_t desc, ml, part, end;
+  size_t ml, part, end;
 };
 inline Split split_area(int ctas, int rows, int hd) {
   Split s;
-  s.desc = kPagedErrBytes;
-  s.ml = s.desc + ((static_cast<size_t>(ctas) * sizeof(int4) + 255) & ~size_t(255));
+  s.ml = (static_cast<size_t>(ctas) * sizeof(int4) + 255) & ~size_t(255);
   s.part = s.ml + ((static_cast<size_t>(ctas) * 2 * rows * sizeof(float2) + 255) & ~size_t(255));
   s.end = s.part + static_cast<size_t>(ctas) * 2 * rows * hd * sizeof(float);
   return s;
 }
-inline void set_split(AttnArgs& a, void* ws, const Split& s) {
-  uint8_t* p = static_cast<uint8_t*>(ws);
-  a.desc = reinterpret_cast<int4*>(p + s.desc);
+inline SplitSet set_split(AttnArgs& a, void* area, int ctas, int row_slots) {
+  const Split s = split_area(ctas, row_slots, a.c.head_dim);
+  uint8_t* p = static_cast<uint8_t*>(area);
+  a.desc = reinterpret_cast<int4*>(p);
   a.ml = reinterpret_cast<float2*>(p + s.ml);
   a.part = reinterpret_cast<float*>(p + s.part);
+  return SplitSet{a.part, a.ml, a.desc, a.by_item, row_slots, 0, 0};
 }
-// joins the split items of a launch (paged_attention.cu): `items` descriptors, `rows` query
-// rows of an item at most (16 or 128 in the partial buffers)
-int launch_combine(const AttnArgs& a, bool bf, int row_slots, int items, int rows, cudaStream_t stream);
-int launch_paged_rows(const AttnArgs& a, int ct, void* ws, int sms, cudaStream_t stream);
-int launch_paged_tiles(const AttnArgs& a, int ct, void* ws, int sms, cudaStream_t stream);
-size_t paged_rows_bytes(int hd, int sms);    // workspace of a form
+int launch_paged_rows(const AttnArgs& a, int ct, void* area, int sms, cudaStream_t stream, SplitSet* set);
+// after_rows: the rows form's kernel was launched just before and may still run
+int launch_paged_tiles(const AttnArgs& a, int ct, void* area, uint32_t* err, int sms, bool after_rows, cudaStream_t stream,
+                       SplitSet* set);
+size_t paged_rows_bytes(int hd, int sms);    // workspace of a form, a multiple of 256
 size_t paged_tiles_bytes(int hd, int sms);
 
 }  // namespace tlx

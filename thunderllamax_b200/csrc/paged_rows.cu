@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel
 constexpr int kRowsCtasPerSm = 4;
 
 template <int CT, int HD>
-int launch_rows(AttnArgs a, void* ws, int sms, cudaStream_t s) {
+int launch_rows(AttnArgs a, void* area, int sms, cudaStream_t s, SplitSet* set) {
   using C = RowsCfg<CT, HD>;
   static bool configured = false;
   if (!configured) {
@@ -459,24 +459,30 @@ int launch_rows(AttnArgs a, void* ws, int sms, cudaStream_t s) {
     configured = true;
   }
   const int ctas = sms * C::kCtas;
-  set_split(a, ws, split_area(ctas, kRowsMax, HD));
   const int64_t items = static_cast<int64_t>(a.n_req) * a.c.kv_heads;
   a.by_item = items <= ctas;
+  *set = set_split(a, area, ctas, kRowsMax);
+  set->items = static_cast<int>(std::min<int64_t>(items, ctas));
+  set->rows = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(a.max_new) * a.group, kRowsMax));
   paged_rows_kernel<CT, HD><<<ctas, 128, C::kSmem, s>>>(a);
-  if (cudaGetLastError() != cudaSuccess) return TLX_ERR_LAUNCH;
-  const int most = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(a.max_new) * a.group, kRowsMax));
-  return launch_combine(a, CT == CT_BF16, kRowsMax, static_cast<int>(std::min<int64_t>(items, ctas)), most, s);
+  return cudaGetLastError() == cudaSuccess ? TLX_OK : TLX_ERR_LAUNCH;
 }
 
 }  // namespace
 
-int launch_paged_rows(const AttnArgs& a, int ct, void* ws, int sms, cudaStream_t s) {
-  const int hd = a.c.head_dim;
-  if (ct == CT_F16) return hd == 256 ? launch_rows<CT_F16, 256>(a, ws, sms, s) : hd == 128 ? launch_rows<CT_F16, 128>(a, ws, sms, s) : launch_rows<CT_F16, 64>(a, ws, sms, s);
-  if (ct == CT_BF16) return hd == 256 ? launch_rows<CT_BF16, 256>(a, ws, sms, s) : hd == 128 ? launch_rows<CT_BF16, 128>(a, ws, sms, s) : launch_rows<CT_BF16, 64>(a, ws, sms, s);
-  return hd == 256 ? launch_rows<CT_Q8, 256>(a, ws, sms, s) : hd == 128 ? launch_rows<CT_Q8, 128>(a, ws, sms, s) : launch_rows<CT_Q8, 64>(a, ws, sms, s);
+template <int CT>
+static int launch_rows_hd(const AttnArgs& a, void* area, int sms, cudaStream_t stream, SplitSet* set) {
+  if (a.c.head_dim == 256) return launch_rows<CT, 256>(a, area, sms, stream, set);
+  if (a.c.head_dim == 128) return launch_rows<CT, 128>(a, area, sms, stream, set);
+  return launch_rows<CT, 64>(a, area, sms, stream, set);
 }
 
-size_t paged_rows_bytes(int hd, int sms) { return split_area(sms * kRowsCtasPerSm, kRowsMax, hd).end; }
+int launch_paged_rows(const AttnArgs& a, int ct, void* area, int sms, cudaStream_t stream, SplitSet* set) {
+  if (ct == CT_F16) return launch_rows_hd<CT_F16>(a, area, sms, stream, set);
+  if (ct == CT_BF16) return launch_rows_hd<CT_BF16>(a, area, sms, stream, set);
+  return launch_rows_hd<CT_Q8>(a, area, sms, stream, set);
+}
+
+size_t paged_rows_bytes(int hd, int sms) { return (split_area(sms * kRowsCtasPerSm, kRowsMax, hd).end + 255) & ~size_t(255); }
 
 }  // namespace tlx

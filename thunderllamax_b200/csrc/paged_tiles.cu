@@ -260,7 +260,10 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
   });
   if (tid == 0) a.desc[blockIdx.x] = make_int4(-1, -1, 0, 0);
   const int n = static_cast<int>(st.u1 - st.u0);
-  if (n == 0) return;
+  if (n == 0) {
+    griddep_wait();
+    return;
+  }
   const uint32_t sbase = smem_u32(sm);
   if (sbase & 1023u) {   // the descriptors need the swizzle atoms' alignment
     if (tid == 0) atomicOr(err, ERR_BAD_PARAM);
@@ -904,6 +907,9 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
     tc_after();
     tc_dealloc(tmem, C::kTmem);
   }
+  // The rows form's kernel may run beside this one; the joining kernel waits for this one
+  // only, so this one does not end before it.
+  griddep_wait();
 }
 
 // The pool as TMA sees it: [page][head][slot][dim], a box of 64 dims (int8: the row) of the
@@ -938,7 +944,7 @@ bool page_map(CUtensorMap* map, const tlx_paged_kv& c, const void* base, const i
 }
 
 template <int CT, int HD>
-int launch_tiles(AttnArgs a, void* ws, int sms, cudaStream_t s) {
+int launch_tiles(AttnArgs a, void* area, uint32_t* err, int sms, bool after_rows, cudaStream_t stream, SplitSet* set) {
   using C = TilesCfg<CT, HD>;
   static bool configured = false;
   if (!configured) {
@@ -950,24 +956,47 @@ int launch_tiles(AttnArgs a, void* ws, int sms, cudaStream_t s) {
     configured = true;
   }
   const int ctas = sms * C::kCtas;
-  set_split(a, ws, split_area(ctas, 128, HD));
   a.by_item = 0;
+  *set = set_split(a, area, ctas, 128);
+  set->items = ctas;
+  set->rows = 128;
   CUtensorMap km, vm;
   if (!page_map(&km, a.c, a.c.k, a.c.k_stride) || !page_map(&vm, a.c, a.c.v, a.c.v_stride)) return TLX_ERR_LAUNCH;
-  paged_tiles_kernel<CT, HD><<<ctas, C::kThreads, C::kSmem, s>>>(a, km, vm, static_cast<uint32_t*>(ws));
-  if (cudaGetLastError() != cudaSuccess) return TLX_ERR_LAUNCH;
-  return launch_combine(a, CT == CT_BF16, 128, ctas, 32, s);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(C::kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = after_rows ? 1 : 0;
+  void* args[] = {&a, &km, &vm, &err};
+  return cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(paged_tiles_kernel<CT, HD>), args) == cudaSuccess
+             ? TLX_OK
+             : TLX_ERR_LAUNCH;
 }
 
 }  // namespace
 
-int launch_paged_tiles(const AttnArgs& a, int ct, void* ws, int sms, cudaStream_t s) {
-  const int hd = a.c.head_dim;
-  if (ct == CT_F16) return hd == 256 ? launch_tiles<CT_F16, 256>(a, ws, sms, s) : hd == 128 ? launch_tiles<CT_F16, 128>(a, ws, sms, s) : launch_tiles<CT_F16, 64>(a, ws, sms, s);
-  if (ct == CT_BF16) return hd == 256 ? launch_tiles<CT_BF16, 256>(a, ws, sms, s) : hd == 128 ? launch_tiles<CT_BF16, 128>(a, ws, sms, s) : launch_tiles<CT_BF16, 64>(a, ws, sms, s);
-  return hd == 256 ? launch_tiles<CT_Q8, 256>(a, ws, sms, s) : hd == 128 ? launch_tiles<CT_Q8, 128>(a, ws, sms, s) : launch_tiles<CT_Q8, 64>(a, ws, sms, s);
+template <int CT>
+static int launch_tiles_hd(const AttnArgs& a, void* area, uint32_t* err, int sms, bool after_rows, cudaStream_t stream,
+                           SplitSet* set) {
+  if (a.c.head_dim == 256) return launch_tiles<CT, 256>(a, area, err, sms, after_rows, stream, set);
+  if (a.c.head_dim == 128) return launch_tiles<CT, 128>(a, area, err, sms, after_rows, stream, set);
+  return launch_tiles<CT, 64>(a, area, err, sms, after_rows, stream, set);
 }
 
-size_t paged_tiles_bytes(int hd, int sms) { return split_area(sms * (hd == 256 ? 1 : 2), 128, hd).end; }   // kCtas at most
+int launch_paged_tiles(const AttnArgs& a, int ct, void* area, uint32_t* err, int sms, bool after_rows, cudaStream_t stream,
+                       SplitSet* set) {
+  if (ct == CT_F16) return launch_tiles_hd<CT_F16>(a, area, err, sms, after_rows, stream, set);
+  if (ct == CT_BF16) return launch_tiles_hd<CT_BF16>(a, area, err, sms, after_rows, stream, set);
+  return launch_tiles_hd<CT_Q8>(a, area, err, sms, after_rows, stream, set);
+}
+
+size_t paged_tiles_bytes(int hd, int sms) {
+  return (split_area(sms * (hd == 256 ? 1 : 2), 128, hd).end + 255) & ~size_t(255);   // kCtas at most
+}
 
 }  // namespace tlx
