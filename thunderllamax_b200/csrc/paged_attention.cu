@@ -128,10 +128,16 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constan
 }
 
 int sm_count() {
-  int dev = 0, n = 0;
+  static int counts[64] = {};   // by device (asking takes as long as a launch)
+  int dev = 0;
   cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n > 0 ? n : 148;
+  if (dev < 0 || dev >= 64) return 148;
+  if (counts[dev] == 0) {
+    int n = 0;
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    counts[dev] = n > 0 ? n : 148;
+  }
+  return counts[dev];
 }
 
 template <bool BF>

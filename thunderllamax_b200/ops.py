@@ -29,6 +29,12 @@ def _stream(t=None):
     return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
 
 
+def _raw_stream(t) -> int:
+    """The current stream of t's device as an integer, without building a Stream object
+    (about 3 us a call, a third of a short kernel's whole call)."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
 def require_device():
     if not torch.cuda.is_available():
         raise TLXError("no CUDA device: the verify path has no CPU implementation")

@@ -41,6 +41,7 @@ class Plan:
         buf = torch.zeros(3 * self.requests + 1 + 2 * self.tokens, dtype=torch.int32, device=device)
         r, t = self.requests, self.tokens
         self.q_start, self.kv_len, self.status, self.slots, self.positions = buf.split([r + 1, r, r, t, t])
+        self._out = tuple(x.data_ptr() for x in (self.q_start, self.kv_len, self.slots, self.positions, self.status))
 
 
 class PageTable:
@@ -65,6 +66,9 @@ class PageTable:
         _i32(self.free, self.pages, "free")
         _i32(self.n_free, 1, "n_free")
         self.ws = ops.Workspace(int(_lib.lib().tlx_paged_plan_workspace_bytes()), self.table.device)
+        # (its own buffers' addresses do not change)
+        self._call, self._ws = _lib.lib().tlx_paged_plan, (self.ws.buf.data_ptr(), self.ws.nbytes)
+        self._table = (self.table.data_ptr(), self.table.stride(0), self.width)
 
     def plan(self, cached_len: torch.Tensor, new_len: torch.Tensor, plan: Plan, held_out: torch.Tensor = None,
              n_free_out: torch.Tensor = None) -> Plan:
@@ -77,12 +81,10 @@ class PageTable:
         _i32(new_len, n, "new_len")
         held_out = self.held if held_out is None else _i32(held_out, n, "held_out")
         n_free_out = self.n_free if n_free_out is None else _i32(n_free_out, 1, "n_free_out")
-        rc = _lib.lib().tlx_paged_plan(
-            cached_len.data_ptr(), new_len.data_ptr(), n, self.page_size, self.table.data_ptr(), self.table.stride(0),
-            self.width, self.held.data_ptr(), held_out.data_ptr(), self.free.data_ptr(), self.pages,
-            self.n_free.data_ptr(), n_free_out.data_ptr(), plan.tokens, plan.q_start.data_ptr(),
-            plan.kv_len.data_ptr(), plan.slots.data_ptr(), plan.positions.data_ptr(), plan.status.data_ptr(),
-            self.ws.buf.data_ptr(), self.ws.nbytes, ops._stream(self.table))
+        rc = self._call(
+            cached_len.data_ptr(), new_len.data_ptr(), n, self.page_size, *self._table, self.held.data_ptr(),
+            held_out.data_ptr(), self.free.data_ptr(), self.pages, self.n_free.data_ptr(), n_free_out.data_ptr(),
+            plan.tokens, *plan._out, *self._ws, ops._raw_stream(self.table))
         check(rc, "paged_plan")
         return plan
 
@@ -94,7 +96,7 @@ class PageTable:
         _i32(done, 1, "done")
         check(_lib.lib().tlx_paged_release(done.data_ptr(), n, self.table.data_ptr(), self.table.stride(0), self.width,
                                            self.held.data_ptr(), self.free.data_ptr(), self.pages,
-                                           self.n_free.data_ptr(), ops._stream(self.table)), "paged_release")
+                                           self.n_free.data_ptr(), ops._raw_stream(self.table)), "paged_release")
 
 
 class PagedCache:
@@ -146,7 +148,7 @@ class PagedCache:
         n = k.shape[0]
         _i32(slots, n, "slots")
         rc = _lib.lib().tlx_paged_append(self._ref, k.data_ptr(), v.data_ptr(), ops._DT[k.dtype], k.stride(0),
-                                         k.stride(1), v.stride(0), v.stride(1), slots.data_ptr(), n, ops._stream(k))
+                                         k.stride(1), v.stride(0), v.stride(1), slots.data_ptr(), n, ops._raw_stream(k))
         check(rc, "paged_append")
 
 
@@ -161,6 +163,8 @@ class PagedAttention:
         if nb == 0:
             raise TLXError(f"unsupported heads: {heads} query, {kv_heads} KV, dim {head_dim}")
         self.ws = ops.Workspace(nb, device)
+        self.scale = self.head_dim ** -0.5
+        self._call, self._ws = _lib.lib().tlx_paged_attention, self.ws.buf.data_ptr()
 
     def __call__(self, cache: PagedCache, table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor,
                  q: torch.Tensor, gate: torch.Tensor = None, scale: float = None, max_new: int = None,
@@ -169,29 +173,35 @@ class PagedAttention:
         tokens sees keys 0 .. kv_len[b] - n + t.  gate: out is multiplied by its sigmoid.
         scale defaults to head_dim ** -0.5.  max_new: the most new tokens of any request
         (default: the number of rows)."""
-        n = q.shape[0]
+        shape, dt = q.shape, cache.q_dtype
         if out is None:
-            out = torch.empty((n, self.heads, self.head_dim), dtype=q.dtype, device=q.device)
-        for t, name in ((q, "q"), (out, "out"), (gate, "gate")):
-            if t is not None and (t.shape != (n, self.heads, self.head_dim) or t.stride(2) != 1 or
-                                  t.dtype != cache.q_dtype or t.device != cache.k.device):
-                raise TLXError(f"{name} must be {cache.q_dtype} [tokens, {self.heads}, {self.head_dim}] rows on the "
-                               "cache's device")
+            out = torch.empty(shape, dtype=dt, device=q.device)
+        dev = cache.k.device
+        if (len(shape) != 3 or shape[1] != self.heads or shape[2] != self.head_dim or q.dtype != dt or
+                q.device != dev or out.shape != shape or out.dtype != dt or out.device != dev):
+            raise TLXError(f"q and out must be {dt} [tokens, {self.heads}, {self.head_dim}] rows on the cache's device")
+        n, (qt, qh, q1), (ot, oh, o1) = shape[0], q.stride(), out.stride()
+        gp, gt, gh, g1 = None, 0, 0, 1
+        if gate is not None:
+            if gate.shape != shape or gate.dtype != dt or gate.device != dev:
+                raise TLXError("gate must be rows like q's")
+            gp, (gt, gh, g1) = gate.data_ptr(), gate.stride()
+        if q1 != 1 or o1 != 1 or g1 != 1:
+            raise TLXError("the rows of q, out and gate must be contiguous")
         if cache.kv_heads != self.kv_heads or cache.head_dim != self.head_dim:
             raise TLXError("the cache has other heads than this attention")
-        if table.dtype != torch.int32 or table.dim() != 2 or table.stride(1) != 1 or table.device != cache.k.device:
+        if table.dtype != torch.int32 or table.dim() != 2 or table.device != dev or table.stride(1) != 1:
             raise TLXError("table must be a row-major int32 [requests, width] tensor on the cache's device")
         r = kv_len.numel()
         if table.shape[0] < r:
             raise TLXError(f"the table has {table.shape[0]} rows for {r} requests")
         _i32(kv_len, 1, "kv_len")
         _i32(q_start, r + 1, "q_start")
-        gp, gs = (gate.data_ptr(), gate.stride()) if gate is not None else (None, (0, 0))
-        rc = _lib.lib().tlx_paged_attention(
+        rc = self._call(
             cache._ref, table.data_ptr(), table.stride(0), table.shape[1], q_start.data_ptr(), kv_len.data_ptr(), r,
-            q.data_ptr(), ops._DT[q.dtype], q.stride(0), q.stride(1), self.heads, n, n if max_new is None else max_new,
-            self.head_dim ** -0.5 if scale is None else scale, gp, gs[0], gs[1], out.data_ptr(), out.stride(0),
-            out.stride(1), self.ws.buf.data_ptr(), self.ws.nbytes, ops._stream(q))
+            q.data_ptr(), ops._DT[dt], qt, qh, self.heads, n, n if max_new is None else max_new,
+            self.scale if scale is None else scale, gp, gt, gh, out.data_ptr(), ot, oh, self._ws, self.ws.nbytes,
+            ops._raw_stream(q))
         check(rc, "paged_attention")
         return out
 

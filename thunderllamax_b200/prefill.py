@@ -163,9 +163,8 @@ def add_rms_norm_q8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tenso
     sx fp32 [m, k/128]): the tokens w4a8_gate_up reads.  x and residual are fp16, bf16 or fp32
     [tokens, k] rows, weight fp32 [k]; residual None: h = x; out may be the residual itself; rs (optional,
     int32 [m, k/128]) receives the chunk sums."""
-    ops.require_device()
-    if x.dim() != 2 or x.stride(1) != 1 or x.dtype not in ops._DT:
-        raise TLXError("x must be a row-major fp16, bf16 or fp32 [tokens, k] tensor")
+    if x.dim() != 2 or x.stride(1) != 1 or x.dtype not in ops._DT or not x.is_cuda:
+        raise TLXError("x must be a row-major fp16, bf16 or fp32 [tokens, k] CUDA tensor")
     m, k = x.shape
     if residual is not None and (residual.shape != x.shape or residual.stride(1) != 1 or
                                  residual.dtype not in ops._DT or residual.device != x.device):
@@ -190,7 +189,7 @@ def add_rms_norm_q8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tenso
                                         None if residual is None else residual.data_ptr(), ops._DT[h_dtype],
                                         0 if residual is None else residual.stride(0), weight.data_ptr(), eps, m, k,
                                         out.data_ptr(), out.stride(0), xq.data_ptr(), xq.stride(0), sx.data_ptr(),
-                                        None if rs is None else rs.data_ptr(), ops._stream(x))
+                                        None if rs is None else rs.data_ptr(), ops._raw_stream(x))
     check(rc, "add_rms_norm_q8")
     return out, xq, sx
 
