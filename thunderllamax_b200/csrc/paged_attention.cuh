@@ -51,12 +51,15 @@ __device__ __forceinline__ Req get_req(const AttnArgs& a, int b) {
   return r;
 }
 
-// units of a request in the rows form: kv_heads items of the same keys (an item without
-// keys is one unit, which writes zeros)
+// Work is dealt in a row of positions in which every item takes kItemCost positions (its
+// Q load, its rows' end) and then one for each unit.  A CTA has the units whose positions
+// lie in its range; both neighbours of a boundary find the same one.
+//
+// units of an item of the rows form (an item without keys is one unit, which writes zeros)
 template <int KT>
 __device__ __forceinline__ int rows_units(const AttnArgs& a, const Req& r) {
   if (r.n < 1 || r.n * static_cast<int64_t>(a.group) > a.rows_limit) return 0;
-  return max(1, (r.keys + KT - 1) / KT) * a.c.kv_heads;
+  return max(1, (r.keys + KT - 1) / KT);
 }
 
 __device__ __forceinline__ int64_t range_start(int64_t units, int cta, int ctas) { return units * cta / ctas; }
@@ -67,14 +70,14 @@ __device__ __forceinline__ int range_of(int64_t units, int64_t u, int ctas) {
   return c;
 }
 
-// Total units and the request (with the unit inside it) at which this CTA's range starts.
+// All positions, and the request (with the position inside it) at which this CTA's range starts.
 // Every thread of the block calls it; THREADS = blockDim.x; scratch: 8-byte aligned shared
 // memory of THREADS / 4 + 16 bytes, free again after the block's next barrier.
 struct Start {
-  int64_t units, u0, u1;
-  int64_t local;   // unit inside request b
+  int64_t units, u0, u1;   // all positions, this CTA's range
+  int64_t local;           // its start inside request b
   int b;
-  int ctas;        // CTAs that have a unit: an item's pieces are consecutive ones
+  int ctas;                // CTAs that have a range
 };
 template <int THREADS, typename F>
 __device__ __forceinline__ Start find_start(const AttnArgs& a, void* scratch, F units_of) {
@@ -84,7 +87,7 @@ __device__ __forceinline__ Start find_start(const AttnArgs& a, void* scratch, F 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int64_t sum = 0;
   for (int b = tid; b < a.n_req; b += THREADS) sum += units_of(b);
-  int64_t incl = sum;
+  int64_t incl = sum;   // (units_of: positions of a request)
   if (tid == 0) s_b = -1;
   auto scan = [&](int64_t v, int64_t& all) -> int64_t {   // inclusive scan over the block
 #pragma unroll

@@ -13,6 +13,8 @@ namespace {
 // contiguous bytes of its key's row as the B fragments of 2 (16-bit) or 4 (int8) steps,
 // and Q is loaded in the same order.  int8 codes become fp16(code - 128) * scale, rounded
 // once, in registers.
+constexpr int kItemCost = 1;   // positions of an item besides its units (see the schedule)
+
 template <int CT, int HD>
 struct RowsCfg {
   static constexpr bool kQ8 = CT == CT_Q8;
@@ -43,22 +45,17 @@ __global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
 
   griddep_launch_dependents();
-  const Start st = find_start<128>(a, psm, [&](int b) { return static_cast<int64_t>(rows_units<KT>(a, get_req(a, b))); });
+  const Start st = find_start<128>(a, psm, [&](int b) -> int64_t {
+    const int units = rows_units<KT>(a, get_req(a, b));
+    return units ? static_cast<int64_t>(units + kItemCost) * a.c.kv_heads : 0;
+  });
   if (!a.by_item && tid == 0) a.desc[blockIdx.x] = make_int4(-1, -1, 0, 0);
-  const int n_units = static_cast<int>(st.u1 - st.u0);
-  if (n_units == 0) return;
+  if (st.u0 == st.u1) return;
 
   // position in the row of units: request, KV head, unit of the item
   struct Pos {
     int b, head, u, of;
     Req r;
-  };
-  auto seek = [&](Pos& p, int b, int64_t local) {
-    p.b = b;
-    p.r = get_req(a, b);
-    p.of = max(1, (p.r.keys + KT - 1) / KT);
-    p.head = static_cast<int>(local / p.of);
-    p.u = static_cast<int>(local % p.of);
   };
   auto advance = [&](Pos& p) {
     if (++p.u < p.of) return;
@@ -116,9 +113,42 @@ __global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel
     }
   };
 
-  Pos load_at, at;
-  seek(load_at, st.b, st.local);
-  at = load_at;
+  Pos load_at;
+  load_at.b = st.b;
+  load_at.r = get_req(a, st.b);
+  load_at.of = rows_units<KT>(a, load_at.r);
+  load_at.head = static_cast<int>(st.local / (load_at.of + kItemCost));
+  const int into = static_cast<int>(st.local % (load_at.of + kItemCost));
+  load_at.u = max(0, into - kItemCost);
+  int64_t pos = st.u0 + max(0, kItemCost - into);   // of the part's first unit
+  // the units of the range
+  int n_units = 0;
+  {
+    int64_t x = pos;
+    int head = load_at.head, of = load_at.of, b = load_at.b, u = load_at.u;
+    while (x < st.u1) {
+      const int k = static_cast<int>(min(static_cast<int64_t>(of - u), st.u1 - x));
+      n_units += k;
+      x += k + kItemCost;
+      u = 0;
+      if (++head < a.c.kv_heads) {   // the request's other heads are like this one
+        const int span = of + kItemCost;
+        const int skip = static_cast<int>(min(static_cast<int64_t>(a.c.kv_heads - head), max(st.u1 - x, static_cast<int64_t>(0)) / span));
+        n_units += skip * of;
+        x += static_cast<int64_t>(skip) * span;
+        head += skip;
+      }
+      if (head == a.c.kv_heads) {
+        head = 0;
+        do {
+          ++b;
+        } while (b < a.n_req && (of = rows_units<KT>(a, get_req(a, b))) == 0);
+        if (b >= a.n_req) break;
+      }
+    }
+  }
+  if (n_units == 0) return;
+  Pos at = load_at;
   int loaded = 0;
 #pragma unroll
   for (int i = 0; i < C::kStages - 1; ++i) {
@@ -135,6 +165,7 @@ __global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
   int lim0 = 0, lim1 = 0;   // keys that rows g and g + 8 see
   bool first = true;        // the next unit starts an item (or this CTA's part of one)
+  int part_i = 0;           // first unit of the part
   for (int i = 0; i < n_units; ++i) {
     const int stage = i % C::kStages;
     if (first) {
@@ -378,14 +409,14 @@ __global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel
         l0 += ssum[w * 16 + g];
         l1 += ssum[w * 16 + g + 8];
       }
-      const int64_t begin = st.u0 + i - at.u, end = begin + at.of;   // the item's units
-      const bool whole = begin >= st.u0 && end <= st.u1;
+      const int part = i + 1 - part_i, u_first = at.u + 1 - part;   // the units of this part
+      const bool whole = u_first == 0 && part == at.of;
       const int rows = at.r.n * a.group;
-      const int slot = 2 * blockIdx.x + (begin > st.u0 ? 1 : 0);   // a part that the CTA's range starts in, or a later one
+      const int slot = 2 * blockIdx.x + (part_i > 0 ? 1 : 0);   // the CTA's first part, or a later one
       if (tid == 0) {
         const int64_t item = static_cast<int64_t>(at.b) * a.c.kv_heads + at.head;
-        if (begin >= st.u0) {   // the item starts here: where its pieces are, if it is split
-          const int4 d = make_int4(whole ? -1 : slot, whole ? -1 : range_of(st.units, end - 1, st.ctas), at.b << 10 | at.head, 0);
+        if (u_first == 0) {   // the item starts here: where its pieces are, if it is split
+          const int4 d = make_int4(whole ? -1 : slot, whole ? -1 : range_of(st.units, pos + at.of - 1, st.ctas), at.b << 10 | at.head, 0);
           if (a.by_item) a.desc[item] = d;
           else if (!whole) a.desc[blockIdx.x] = d;
         }
@@ -438,6 +469,10 @@ __global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel
           for (int j = 0; j < DB; ++j) put2(8 * j + 2 * q, o[j][2 * half], o[j][2 * half + 1]);
         }
       }
+    }
+    if (first) {
+      pos += i + 1 - part_i + kItemCost;
+      part_i = i + 1;
     }
     if (i + 1 < n_units) advance(at);
   }

@@ -103,6 +103,8 @@ struct TilesCfg {
   static constexpr uint32_t kIdescPV = (1u << 4) | kFmt | (1u << 16) | static_cast<uint32_t>(HD >> 3) << 17 | (128u >> 4) << 24;
 };
 
+constexpr int kItemCost = 6;   // positions of an item besides its units (see the schedule)
+
 // sum over i < n of floor((a i + b) / m): the Euclid-like recursion, as a loop
 __device__ __noinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
   int64_t s = 0;
@@ -140,8 +142,8 @@ __device__ __forceinline__ int tile_keys(const AttnArgs& a, const Req& r, int ti
 __device__ __forceinline__ int tile_units(const AttnArgs& a, const Req& r, int tile) {
   return max(1, (tile_keys(a, r, tile) + 63) >> 6);
 }
-// units of one KV head in the tiles before `tile`
-__device__ __noinline__ int64_t units_before(const AttnArgs& a, const Req& r, int tile) {
+// positions of one KV head in the tiles before `tile`
+__device__ __noinline__ int64_t positions_before(const AttnArgs& a, const Req& r, int tile) {
   const int64_t tt = tile_tokens(a), c = static_cast<int64_t>(r.kv) - r.n_all;
   const int full = min(tile, r.n / static_cast<int>(tt));   // tiles with all their tokens
   int64_t s = 0;
@@ -151,7 +153,7 @@ __device__ __noinline__ int64_t units_before(const AttnArgs& a, const Req& r, in
     i = full;
   }
   for (; i < tile; ++i) s += tile_units(a, r, i);
-  return s;
+  return s + static_cast<int64_t>(tile) * kItemCost;
 }
 
 // Infinite and NaN values of V are replaced by 0 in shared memory in the units that some rows do
@@ -214,6 +216,28 @@ __device__ __forceinline__ Pos item_after(const AttnArgs& a, Pos p) {
   return p;
 }
 
+// units in the positions [pos, end), from unit p.u (at pos) of item p on
+__device__ __noinline__ int units_of_range(const AttnArgs& a, Pos p, int64_t pos, int64_t end) {
+  int n = 0;
+  while (pos < end) {
+    const int k = static_cast<int>(min(static_cast<int64_t>(p.of - p.u), end - pos));
+    n += k;
+    pos += k + kItemCost;
+    p.u = 0;
+    if (p.head + 1 < a.c.kv_heads) {   // the tile's other heads are like this one
+      const int span = p.of + kItemCost;
+      const int skip = static_cast<int>(min(static_cast<int64_t>(a.c.kv_heads - 1 - p.head), max(end - pos, static_cast<int64_t>(0)) / span));
+      n += skip * p.of;
+      pos += static_cast<int64_t>(skip) * span;
+      p.head += skip;
+    }
+    if (pos >= end) break;
+    p = item_after(a, p);
+    if (p.b >= a.n_req) break;
+  }
+  return n;
+}
+
 template <int CT, int HD>
 __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::kCtas)
     paged_tiles_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap k_map,
@@ -244,23 +268,22 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
   // of the softmax)
   volatile int* bad = reinterpret_cast<int*>(tmem_holder + 2);
   struct First {
-    int tile, head, u;
+    int tile, head, u, skip, n;   // ..., positions before the first unit, units of the range
   };
   First* first_at = reinterpret_cast<First*>(tmem_holder + 10);
   volatile float* m_sh = reinterpret_cast<float*>(sm + C::kOffX);   // [128]
   volatile float* l_sh = m_sh + 128;                                 // [2 items][2 groups][128]
-  static_assert((4 * 6 + 25) * 8 + 13 * 4 <= 512 && RING <= 6 && C::kRaw <= 6, "barrier area");
+  static_assert((4 * 6 + 25) * 8 + 15 * 4 <= 512 && RING <= 6 && C::kRaw <= 6, "barrier area");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   griddep_launch_dependents();
   const Start st = find_start<C::kThreads>(a, sm + C::kOffP, [&](int b) -> int64_t {
     const Req r = get_req(a, b);
     const int tiles = tile_count(a, r);
-    return tiles ? units_before(a, r, tiles) * a.c.kv_heads : 0;
+    return tiles ? positions_before(a, r, tiles) * a.c.kv_heads : 0;
   });
   if (tid == 0) a.desc[blockIdx.x] = make_int4(-1, -1, 0, 0);
-  const int n = static_cast<int>(st.u1 - st.u0);
-  if (n == 0) {
+  if (st.u0 == st.u1) {
     griddep_wait();
     return;
   }
@@ -271,19 +294,28 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
   }
   if (warp == 0) {   // the tile, head and unit at which the range starts: a 32-way search
     const Req r = get_req(a, st.b);
-    int lo = 0, hi = tile_count(a, r);   // units_before(lo) * heads <= local < units_before(hi) * heads
+    int lo = 0, hi = tile_count(a, r);   // positions_before(lo) * heads <= local < positions_before(hi) * heads
     while (hi - lo > 1) {
       const int step = (hi - lo + 31) / 32, t = min(lo + lane * step, hi);
-      const bool le = t < hi && units_before(a, r, t) * a.c.kv_heads <= st.local;
+      const bool le = t < hi && positions_before(a, r, t) * a.c.kv_heads <= st.local;
       const int k = 31 - __clz(__ballot_sync(0xffffffffu, le));   // lane 0 always holds
       const int nlo = lo + k * step;
       hi = min(hi, nlo + step);
       lo = nlo;
     }
     if (lane == 0) {
-      const int64_t rest = st.local - units_before(a, r, lo) * a.c.kv_heads;
-      const int of = tile_units(a, r, lo);
-      *first_at = First{lo, static_cast<int>(rest / of), static_cast<int>(rest % of)};
+      const int64_t rest = st.local - positions_before(a, r, lo) * a.c.kv_heads;
+      Pos p;
+      p.b = st.b;
+      p.r = r;
+      p.tiles = tile_count(a, r);
+      p.tile = lo;
+      p.of = tile_units(a, r, lo);
+      p.head = static_cast<int>(rest / (p.of + kItemCost));
+      const int into = static_cast<int>(rest % (p.of + kItemCost));
+      p.u = max(0, into - kItemCost);
+      const int64_t pos = st.u0 + max(0, kItemCost - into);
+      *first_at = First{p.tile, p.head, p.u, static_cast<int>(pos - st.u0), units_of_range(a, p, pos, st.u1)};
     }
   }
   if (tid == 0) {
@@ -326,6 +358,7 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
   at.tile = first_at->tile;
   at.head = first_at->head;
   at.u = first_at->u;
+  const int n = first_at->n;
   at.of = tile_units(a, at.r, at.tile);
   // the next item (not called past the last unit of the launch)
   auto next_item = [&](Pos& p) { p = item_after(a, p); };
@@ -379,6 +412,7 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
       if (lane == 0) mbar_arrive(q_full);
     };
     int i = 0, item = -1, last = -1, begin_i = 0;
+    int64_t pos = st.u0 + first_at->skip;   // of the part's first unit
     Pos next = at;
     float m_ref, l_run;
     for (;;) {
@@ -412,11 +446,11 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
         }
         if (!(ok = warp_wait(&pv_done[last & 1], (last >> 1) & 1))) break;
         tc_after();
-        const int64_t begin = st.u0 + begin_i - at.u, end = begin + at.of;   // the item's units
-        const bool whole = begin >= st.u0 && end <= st.u1;
-        const int slot = 2 * blockIdx.x + (begin > st.u0 ? 1 : 0);
-        if (tid == 0 && begin >= st.u0 && !whole)
-          a.desc[blockIdx.x] = make_int4(slot, range_of(st.units, end - 1, st.ctas), at.b << 10 | at.head, at.tile);
+        const bool whole = at.u == 0 && last + 1 - begin_i == at.of;
+        const int slot = 2 * blockIdx.x + (begin_i > 0 ? 1 : 0);   // the CTA's first part, or a later one
+        if (tid == 0 && at.u == 0 && !whole)
+          a.desc[blockIdx.x] = make_int4(slot, range_of(st.units, pos + at.of - 1, st.ctas), at.b << 10 | at.head, at.tile);
+        pos += last + 1 - begin_i + kItemCost;
         if (any) {
           const bool sees = lim > 0;
           const float inv = 1.f / l_run;
