@@ -41,6 +41,21 @@ template <int N>
 __device__ __forceinline__ void reg_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N));
 }
+// two fp32 operations an instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n"
+      : "=l"(*reinterpret_cast<uint64_t*>(&d))
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)), "l"(*reinterpret_cast<uint64_t*>(&c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;\n"
+      : "=l"(*reinterpret_cast<uint64_t*>(&d))
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return d;
+}
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* b) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(
@@ -103,7 +118,7 @@ struct TilesCfg {
   static constexpr uint32_t kIdescPV = (1u << 4) | kFmt | (1u << 16) | static_cast<uint32_t>(HD >> 3) << 17 | (128u >> 4) << 24;
 };
 
-constexpr int kItemCost = 6;   // positions of an item besides its units (see the schedule)
+constexpr int kItemCost = 8;   // positions of an item besides its units (see the schedule)
 
 // sum over i < n of floor((a i + b) / m): the Euclid-like recursion, as a loop
 __device__ __noinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
@@ -456,46 +471,46 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
           const float inv = 1.f / l_run;
           const int64_t tok = at.r.q0 + t;
           const int head = at.head * a.group + hl;
-          uint4 gn[4];   // the gate's next 32 dims, in flight
-          auto gate_of = [&](int c) {
-            if (!whole || !a.gate || !valid) return;
-            const uint4* gp = reinterpret_cast<const uint4*>(a.gate + tok * a.g_tok + head * a.g_head + c * 32);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) gn[j] = __ldg(gp + j);
-          };
-          gate_of(grp * (HD / 32 / NG));
+          const uint16_t* g_row = a.gate + tok * a.g_tok + head * a.g_head;
+          uint16_t* o_row = a.out + tok * a.o_tok + head * a.o_head;
+          float* p_row = a.part + (static_cast<int64_t>(slot) * 128 + row) * HD;
+          const bool gate = whole && a.gate && valid;
+          uint4 g0, g1;   // the gate's next 16 dims, in flight
+          constexpr int CN = HD / 16 / NG;
+          if (gate) {
+            g0 = __ldg(reinterpret_cast<const uint4*>(g_row + grp * CN * 16));
+            g1 = __ldg(reinterpret_cast<const uint4*>(g_row + grp * CN * 16 + 8));
+          }
 #pragma unroll 1
-          for (int c = grp * (HD / 32 / NG); c < (grp + 1) * (HD / 32 / NG); ++c) {
-            uint4 gv[4] = {gn[0], gn[1], gn[2], gn[3]};
-            if (c + 1 < (grp + 1) * (HD / 32 / NG)) gate_of(c + 1);
-            uint32_t r[32];
-            tc_ld32(tmem + lanes + C::kColO + c * 32, r);
+          for (int c = grp * CN; c < (grp + 1) * CN; ++c) {
+            const uint32_t gw[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
+            if (gate && c + 1 < (grp + 1) * CN) {
+              g0 = __ldg(reinterpret_cast<const uint4*>(g_row + c * 16 + 16));
+              g1 = __ldg(reinterpret_cast<const uint4*>(g_row + c * 16 + 24));
+            }
+            uint32_t r[16];
+            tc_ld16(tmem + lanes + C::kColO + c * 16, r);
             tc_wait_ld();
             if (!valid) continue;
             if (!whole) {
-              float4* dst = reinterpret_cast<float4*>(a.part + (static_cast<int64_t>(slot) * 128 + row) * HD + c * 32);
+              uint4* dst = reinterpret_cast<uint4*>(p_row + c * 16);
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
-                dst[j] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
-                                     __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
+              for (int j = 0; j < 4; ++j) dst[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
             } else {
-              uint4* dst = reinterpret_cast<uint4*>(a.out + tok * a.o_tok + head * a.o_head + c * 32);
+              uint32_t w[8];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                float v[8];
-#pragma unroll
-                for (int x = 0; x < 8; ++x) v[x] = sees ? __uint_as_float(r[8 * j + x]) * inv : 0.f;
-                if (a.gate) {
-                  const uint32_t gw[4] = {gv[j].x, gv[j].y, gv[j].z, gv[j].w};
-#pragma unroll
-                  for (int x = 0; x < 4; ++x) {
-                    const float2 y = unpack2<BF>(gw[x]);
-                    v[2 * x] = gated(v[2 * x], y.x);
-                    v[2 * x + 1] = gated(v[2 * x + 1], y.y);
-                  }
+              for (int j = 0; j < 8; ++j) {
+                float v0 = sees ? __uint_as_float(r[2 * j]) * inv : 0.f, v1 = sees ? __uint_as_float(r[2 * j + 1]) * inv : 0.f;
+                if (gate) {
+                  const float2 y = unpack2<BF>(gw[j]);
+                  v0 = gated(v0, y.x);
+                  v1 = gated(v1, y.y);
                 }
-                dst[j] = make_uint4(pack2<BF>(v[0], v[1]), pack2<BF>(v[2], v[3]), pack2<BF>(v[4], v[5]), pack2<BF>(v[6], v[7]));
+                w[j] = pack2<BF>(v0, v1);
               }
+              uint4* dst = reinterpret_cast<uint4*>(o_row + c * 16);
+              dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+              dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
             }
           }
           if (!whole && valid && grp == 0) a.ml[slot * 128 + row] = make_float2(m_ref, l_run);
@@ -599,18 +614,19 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
         // the P buffer is free once the product that read it is done
         if (i >= PB && !(ok = warp_wait(&pv_done[(i - PB) & 1], ((i - PB) >> 1) & 1))) break;
         if (run) {
-          float sums[4] = {0.f, 0.f, 0.f, 0.f};
+          float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          const float2 sc2 = make_float2(sc, sc), off2 = make_float2(off, off);
           auto weights = [&](const uint32_t (&r)[32], int c) {
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
               uint32_t w[4];
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                // 2^(scale log2(e) s - m): one fma and one ex2; a masked key's -inf gives 0
-                const float p0 = ex2_approx(fmaf(__uint_as_float(r[8 * x + 2 * j]), sc, off));
-                const float p1 = ex2_approx(fmaf(__uint_as_float(r[8 * x + 2 * j + 1]), sc, off));
-                sums[j] += p0 + p1;
-                w[j] = pack2<BF>(p0, p1);
+                // 2^(scale log2(e) s - m); a masked key's -inf gives 0
+                const float2 z = fma2(make_float2(__uint_as_float(r[8 * x + 2 * j]), __uint_as_float(r[8 * x + 2 * j + 1])), sc2, off2);
+                const float2 e = make_float2(ex2_approx(z.x), ex2_approx(z.y));
+                sums[j & 1] = add2(sums[j & 1], e);
+                w[j] = pack2<BF>(e.x, e.y);
               }
               *reinterpret_cast<uint4*>(sm + C::kOffP + pb * C::kPBytes + sw128(row, c * 4 + x)) =
                   make_uint4(w[0], w[1], w[2], w[3]);
@@ -618,7 +634,8 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
           };
           weights(r0, 0);
           weights(r1, 1);
-          l_run += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+          const float2 t2 = add2(sums[0], sums[1]);
+          l_run += t2.x + t2.y;
         }
         fence_proxy_async_smem();
         tc_before();
