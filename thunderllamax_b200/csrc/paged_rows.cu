@@ -193,7 +193,11 @@ __global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel
     }
     cp_async_wait<C::kStages - 2>();
     __syncwarp();
-    const uint8_t* kb = sm + stage * C::kStage;
+    const uint32_t kb = sbase + stage * C::kStage;   // (32-bit shared addresses throughout)
+    // chunk 4 j + q of a row lies at 4 (j ^ (row & 1)) + q, and row & 1 = g & 1: even and odd
+    // j from one address each
+    const uint32_t k_even = kb + (warp * KW + g) * C::kRow + q * 16 + ((Q8 && HD == 64) ? 0 : (g & 1) * 64);
+    const uint32_t k_odd = kb + (warp * KW + g) * C::kRow + q * 16 + 64 - (g & 1) * 64;
     // S of this warp's keys.  K reads: 8 lanes of a phase are 2 keys x 4 chunks, the
     // swizzle puts the second key's chunks in the other half of the banks.
     float s[NB][4];
@@ -203,20 +207,19 @@ __global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel
       float e[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
       if constexpr (Q8) {
         uint32_t sw[HD / 64];   // the row's scales, two groups a word
-        const uint8_t* sp = kb + kOffKs + row * C::kScaleRow;
+        const uint32_t sp = kb + kOffKs + row * C::kScaleRow;
         if constexpr (HD == 256) {
-          const uint4 v = lds128(sp);
+          const uint4 v = ls128(sp);
           sw[0] = v.x; sw[1] = v.y; sw[2] = v.z; sw[3] = v.w;
         } else if constexpr (HD == 128) {
-          const uint2 v = lds64(sp);
+          const uint2 v = ls64(sp);
           sw[0] = v.x; sw[1] = v.y;
         } else {
-          sw[0] = lds32(sp);
+          sw[0] = ls32(sp);
         }
 #pragma unroll
         for (int j = 0; j < HD / 64; ++j) {
-          const int ch = HD == 64 ? q : (4 * j + q) ^ ((row & 1) << 2);
-          const uint4 v = lds128(kb + row * C::kRow + ch * 16);
+          const uint4 v = ls128((j & 1 ? k_odd : k_even) + nb * 8 * C::kRow + (j >> 1) * 128);
           const uint32_t s2 = prmt(sw[j], sw[j], q >= 2 ? 0x3232u : 0x1010u);
           const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -225,7 +228,7 @@ __global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel
       } else {
 #pragma unroll
         for (int j = 0; j < HD / 32; ++j) {
-          const uint4 v = lds128(kb + row * C::kRow + (((4 * j + q) ^ ((row & 1) << 2)) * 16));
+          const uint4 v = ls128((j & 1 ? k_odd : k_even) + nb * 8 * C::kRow + (j >> 1) * 128);
           mma16<BF>(e[0], qf[2 * j], v.x, v.y);
           mma16<BF>(e[1], qf[2 * j + 1], v.z, v.w);
         }
@@ -295,7 +298,7 @@ __global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel
     }
     __syncthreads();   // P is in
     // O of this warp's dims
-    const uint8_t* vb = kb + kOffV;
+    const uint32_t vb = kb + kOffV;
     // A key that some rows do not see must not reach them through 0 * inf or 0 * NaN: units
     // with such keys are looked over first (of single tokens there are none).
     bool slow = false;
@@ -304,10 +307,10 @@ __global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel
       for (int key = max(0, at.r.kv - at.r.n_all + 1 - at.u * KT) + warp; key < KT; key += 4) {
         if constexpr (Q8) {   // (any product may overflow where the scale passes 65504 / 128)
           for (int x = lane; x < HD / 32; x += 32)
-            found |= !(fabsf(__half2float(*reinterpret_cast<const __half*>(kb + kOffVs + key * C::kScaleRow + 2 * x))) < 511.f);
+            found |= !(fabsf(__half2float(__ushort_as_half(static_cast<uint16_t>(ls16(kb + kOffVs + key * C::kScaleRow + 2 * x))))) < 511.f);
         } else {
           for (int x = lane; x < CPR; x += 32) {
-            const uint4 v = lds128(vb + key * C::kRow + x * 16);
+            const uint4 v = ls128(vb + key * C::kRow + x * 16);
             found |= bad16<BF>(v.x) || bad16<BF>(v.y) || bad16<BF>(v.z) || bad16<BF>(v.w);
           }
         }
@@ -344,22 +347,25 @@ __global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel
           // lane (g, q): keys 2q, 2q+1, 2q+8, 2q+9 and DB contiguous dims from DB g on
           uint32_t w[4][DB > 4 ? 2 : 1];
           uint32_t sh[4];
+          // (row >> 1) & 3 = q for all four rows: one address and immediates
+          const int byte = warp * DW + DB * g;
+          const int ch = HD == 64 ? (byte >> 4) ^ q : (byte >> 4) ^ (q << 1);
+          const uint32_t v_at = vb + (k * 16 + 2 * q) * C::kRow + ch * 16 + (byte & 15);
+          const uint32_t s_at = kb + kOffVs + (k * 16 + 2 * q) * C::kScaleRow + (byte >> 5) * 2;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int row = k * 16 + 2 * q + (e & 1) + (e >> 1) * 8;
-            const int byte = warp * DW + DB * g;
-            const int ch = HD == 64 ? (byte >> 4) ^ ((row >> 1) & 3) : (byte >> 4) ^ (((row >> 1) & 3) << 1);
-            const uint8_t* p = vb + row * C::kRow + ch * 16 + (byte & 15);
+            const int row = (e & 1) + (e >> 1) * 8;
+            const uint32_t p = v_at + row * C::kRow;
             if constexpr (DB == 8) {
-              const uint2 v = lds64(p);
+              const uint2 v = ls64(p);
               w[e][0] = v.x;
               w[e][1] = v.y;
             } else if constexpr (DB == 4) {
-              w[e][0] = lds32(p);
+              w[e][0] = ls32(p);
             } else {
-              w[e][0] = *reinterpret_cast<const uint16_t*>(p);
+              w[e][0] = ls16(p);
             }
-            sh[e] = *reinterpret_cast<const uint16_t*>(kb + kOffVs + row * C::kScaleRow + (byte >> 5) * 2);
+            sh[e] = ls16(s_at + row * C::kScaleRow);
           }
           const uint32_t s01 = prmt(sh[0], sh[1], 0x5410u), s23 = prmt(sh[2], sh[3], 0x5410u);
 #pragma unroll
@@ -381,7 +387,7 @@ __global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel
             const int row = k * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
             const int ch = (warp * DB + j + (lane >> 4)) ^ (row & 7);
             uint32_t v[4];
-            ldsm4t(v, smem_u32(vb) + row * C::kRow + ch * 16);
+            ldsm4t(v, vb + row * C::kRow + ch * 16);
             product(j, pf, v[0], v[1], k);
             product(j + 1, pf, v[2], v[3], k);
           }
