@@ -527,15 +527,18 @@ int tlx_paged_append(const tlx_paged_kv* cache, const void* k, const void* v, in
  * first).  Row t of the n = q_start[b + 1] - q_start[b] new tokens of request b sees the
  * keys j <= kv_len[b] - n + t:
  *   out[q_start[b] + t][h] = softmax_j(scale * q . k_j) v_j  (* sigmoid(gate), if given)
- * with query head h on KV head h / (heads / kv_heads), heads / kv_heads <= 128.  A row
- * that sees no key (kv_len 0, say) gives 0; what the pages hold past kv_len is never used.
+ * with query head h on KV head h / (heads / kv_heads), heads / kv_heads <= 128, scale
+ * positive.  A row that sees no key (kv_len 0, say) gives 0; what the pages hold past
+ * kv_len, and a later token's K and V, never reach a row, whatever they are (infinite and
+ * NaN included); a page id outside the pool reads as zero rows.
  * q, gate and out are [n_tokens][heads][head_dim] of one dtype (fp16 or bf16), token and
  * head strides in elements, 16-byte multiples.  fp16 q reads fp16 and TLX_DT_Q8 caches,
  * bf16 q bf16 caches.  max_new: no request has more new tokens (rows past it are not
  * written); n_tokens is always a valid bound.  Softmax statistics and sums are fp32, the
  * probabilities are rounded to the dtype of q for the product with v.  Rows past
  * q_start[n_requests] are not written.  Results do not depend on the order in which the
- * device runs the work.
+ * device runs the work (they do depend, by rounding, on how the keys of a request are cut
+ * into pieces, and so on the whole batch's lengths).
  * Workspace: tlx_paged_attention_workspace_bytes, 256-byte aligned, zeroed once; the first
  * word holds the error bits of bounded waits (tlx_workspace_error). */
 size_t tlx_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim);
@@ -546,7 +549,7 @@ int tlx_paged_attention(const tlx_paged_kv* cache, const int32_t* block_table, i
                         int64_t out_tok_stride, int64_t out_head_stride, void* ws, size_t ws_bytes, void* stream);
 
 /* h = x + residual, y = h * rsqrt(mean(h^2) + eps) * weight, and y in int8 with one scale
- * per (token, 128-k chunk): s = max(max|y|, 1e-6) * (1/127), xq = clamp(rint(y / s)), the
+ * per (token, 128-k chunk): s = max(max|y|, 1e-6) * (1/127), xq = rint(y * (1 / s)), the
  * token format tlx_prefill_w4a8_gate_up reads (tlx_act_quant_q8 quantises fp16 tokens by
  * the same rule).  x is fp16, bf16 or fp32; residual (NULL: h = x) and h_out (NULL: not
  * wanted; may be the residual itself) share r_dtype; weight is fp32.  h, the mean and y

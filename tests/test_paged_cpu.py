@@ -52,7 +52,8 @@ def test_cache_refusals(lib, kw, code):
 @pytest.mark.parametrize("kw,code", [
     (dict(heads=5), SHAPE), (dict(heads=258), SHAPE), (dict(heads=0), SHAPE), (dict(n_req=0), SHAPE),
     (dict(tokens=-1), SHAPE), (dict(most=-1), SHAPE), (dict(width=0), SHAPE), (dict(ld=7), SHAPE),
-    (dict(scale=float("nan")), SHAPE), (dict(dt=F32), DTYPE), (dict(dt=BF16), DTYPE), (dict(table=None), NULL),
+    (dict(scale=float("nan")), SHAPE), (dict(scale=0.0), SHAPE), (dict(scale=-0.1), SHAPE), (dict(scale=float("inf")), SHAPE),
+    (dict(dt=F32), DTYPE), (dict(dt=BF16), DTYPE), (dict(table=None), NULL),
     (dict(q_start=None), NULL), (dict(kv=None), NULL), (dict(q=None), NULL), (dict(out=None), NULL),
     (dict(ws=None), NULL), (dict(q=P + 2), ALIGN), (dict(qt=513), ALIGN), (dict(oh=129), ALIGN), (dict(ws=P + 16), ALIGN),
     (dict(gate=P + 8), ALIGN), (dict(gate=P, gt=4), ALIGN), (dict(ws_bytes=8), WORKSPACE), (dict(tokens=0), OK),

@@ -13,6 +13,8 @@
 //   tokens, a few drafts): bound by the cache's bytes, so a warp-level matrix product on
 //   16 rows is enough and the decoded keys never leave registers.
 // tiles form (paged_tiles_kernel)  the rest: tcgen05 on tiles of 128 query rows.
+#include <cmath>
+
 #include "paged_attention.cuh"
 
 namespace tlx {
@@ -190,7 +192,7 @@ int tlx_paged_attention(const tlx_paged_kv* cache, const int32_t* block_table, i
   const int rc = check_paged_kv(cache);
   if (rc) return rc;
   if (n_tokens < 0 || n_tokens > (1 << 28) || n_requests < 1 || n_requests > (1 << 20) || max_new < 0 ||
-      table_width < 1 || table_stride < table_width || !(scale == scale))
+      table_width < 1 || table_stride < table_width || !(scale > 0.f && scale < INFINITY))
     return TLX_ERR_SHAPE;
   const size_t need = tlx_paged_attention_workspace_bytes(heads, cache->kv_heads, cache->head_dim);
   if (!need) return TLX_ERR_SHAPE;
