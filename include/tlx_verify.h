@@ -551,10 +551,10 @@ int tlx_paged_attention(const tlx_paged_kv* cache, const int32_t* block_table, i
 /* h = x + residual, y = h * rsqrt(mean(h^2) + eps) * weight, and y in int8 with one scale
  * per (token, 128-k chunk): s = max(max|y|, 1e-6) * (1/127), xq = rint(y * (1 / s)), the
  * token format tlx_prefill_w4a8_gate_up reads (tlx_act_quant_q8 quantises fp16 tokens by
- * the same rule).  x is fp16, bf16 or fp32; residual (NULL: h = x) and h_out (NULL: not
- * wanted; may be the residual itself) share r_dtype; weight is fp32.  h, the mean and y
- * stay in fp32; h is rounded once when it is stored.  rs (optional) receives the chunk
- * sums.  k % 128 == 0, k <= 32768; rows are 16-byte aligned (xq: 8). */
+ * the same rule with the IEEE quotient).  x is fp16, bf16 or fp32; residual (NULL: h = x)
+ * and h_out (NULL: not wanted; may be the residual itself) share r_dtype; weight is fp32.
+ * h, the mean and y stay in fp32; h is rounded once when it is stored.  A NaN gives its row
+ * NaN scales.  rs (optional) receives the chunk sums.  k % 128 == 0, k <= 32768; rows are 16-byte aligned (xq: 8). */
 int tlx_add_rms_norm_q8(const void* x, int x_dtype, int64_t ldx, const void* residual, int r_dtype, int64_t ldr,
                         const float* weight, float eps, int m, int64_t k, void* h_out, int64_t ldh, int8_t* xq,
                         int64_t ldq, float* sx, int32_t* rs, void* stream);

@@ -28,6 +28,8 @@ BAD_CACHES = [(dict(k=None), NULL), (dict(dt=F32), DTYPE), (dict(dt=Q8), NULL), 
               (dict(page=24), SHAPE), (dict(page=4), SHAPE), (dict(page=2048), SHAPE), (dict(pages=0), SHAPE),
               (dict(pages=1 << 30), SHAPE), (dict(heads=0), SHAPE), (dict(k=P + 2), ALIGN),
               (dict(stride=(64 * 128 * 2, 64 * 128, 129)), ALIGN), (dict(stride=(-8, 8, 128)), SHAPE),
+              (dict(stride=(64 * 128 * 2, 0, 128)), SHAPE), (dict(stride=(1 << 40, 64 * 128, 128)), SHAPE),
+              (dict(dt=Q8, ks=P, vs=P, sstride=(512, 0, 4)), SHAPE),
               (dict(dt=Q8, ks=P + 2, vs=P, sstride=(512, 256, 4)), ALIGN),
               (dict(dt=Q8, ks=P, vs=P, sstride=(512, 255, 4)), ALIGN)]
 

@@ -29,10 +29,14 @@ inline int check_paged_kv(const tlx_paged_kv* c) {
   if ((reinterpret_cast<uintptr_t>(c->k) & 15) || (reinterpret_cast<uintptr_t>(c->v) & 15)) return TLX_ERR_ALIGN;
   if (q8 && ((reinterpret_cast<uintptr_t>(c->k_scale) % sbytes) || (reinterpret_cast<uintptr_t>(c->v_scale) % sbytes)))
     return TLX_ERR_ALIGN;
+  const int64_t count[3] = {c->pages, c->kv_heads, c->page_size};
+  const int64_t most = (int64_t(1) << 40) / esz;   // a TMA stride's limit
   for (int i = 0; i < 3; ++i) {
-    if (c->k_stride[i] < 0 || c->v_stride[i] < 0) return TLX_ERR_SHAPE;
+    const int64_t least = count[i] > 1 ? 1 : 0;    // rows that share memory cannot be a cache
+    if (c->k_stride[i] < least || c->v_stride[i] < least || c->k_stride[i] >= most || c->v_stride[i] >= most)
+      return TLX_ERR_SHAPE;
     if (((c->k_stride[i] * esz) & 15) || ((c->v_stride[i] * esz) & 15)) return TLX_ERR_ALIGN;
-    if (q8 && (c->ks_stride[i] < 0 || c->vs_stride[i] < 0)) return TLX_ERR_SHAPE;
+    if (q8 && (c->ks_stride[i] < least || c->vs_stride[i] < least)) return TLX_ERR_SHAPE;
     if (q8 && ((c->ks_stride[i] * 2) % sbytes || (c->vs_stride[i] * 2) % sbytes)) return TLX_ERR_ALIGN;
   }
   return TLX_OK;
