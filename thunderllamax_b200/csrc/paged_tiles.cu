@@ -30,6 +30,12 @@ namespace {
 // Every wait is bounded: a timeout raises the error word, all roles leave, issued MMAs
 // and copies are drained and tensor memory is freed.
 //
+// Measured (24 / 4 heads, dim 256): 4096 new tokens over 8192 fp16 keys 0.68 to 0.76 ms with
+// the power cap's clocks (0.81 PFLOP/s, 0.49 of the measured matrix rate); the MMAs alone
+// would take 0.43 ms in this form (16 MMAs of N = 64 and 4 of N = 256 cost 1050 to 1430
+// cycles a unit from one or two issuers); 11 rows at 100011 int8 keys 135 us (1.6 TB/s; the
+// converters are the longest loop); the mixed bf16 batch 208 us.
+//
 // Code size: the roles' loops run side by side on each scheduler, one warp each, so what
 // does not fit the instruction caches is fetched again for every unit.  Hence the loops
 // that could be unrolled further and are not, and one call site for each large body.
@@ -118,7 +124,9 @@ struct TilesCfg {
   static constexpr uint32_t kIdescPV = (1u << 4) | kFmt | (1u << 16) | static_cast<uint32_t>(HD >> 3) << 17 | (128u >> 4) << 24;
 };
 
-constexpr int kItemCost = 8;   // positions of an item besides its units (see the schedule)
+// Positions of an item besides its units (see the schedule): with 3 / 6 / 10 the mixed batch
+// takes 309 / 250 / 246 us, with none 440.
+constexpr int kItemCost = 8;
 
 // sum over i < n of floor((a i + b) / m): the Euclid-like recursion, as a loop
 __device__ __noinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
