@@ -778,6 +778,7 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
       constexpr int ATOMS = Q8 ? 1 : HD / 64, LR = Q8 ? C::kRaw : RING, NL = C::kLoaders;
       const int rows = min(a.c.page_size, 64), box = lane * NL + warp - C::kLoadWarp, part = box / ATOMS, atom = box % ATOMS;
       const bool mine = part * rows < 64;
+      const int row_bits = min(a.shift, 6);   // log2(rows)
       // bytes of this warp's boxes
       const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine)) * rows * (Q8 ? HD : 128);
       // Page ids come from two windows of 32 table entries, a lane holding one of each: the
@@ -813,16 +814,18 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
                           : sm + slot * C::kHalf + atom * 8192 + part * rows * 128;
         if (mine) tma_load_4d(dst, v ? &v_map : &k_map, atom * 64, in, head, page, &landed[slot]);
         if constexpr (Q8) {
-          const uint16_t* sc = static_cast<const uint16_t*>(v ? a.c.v_scale : a.c.k_scale);
-          const int64_t* ss = v ? a.c.vs_stride : a.c.ks_stride;
-          const uint32_t sb = sbase + C::kOffRaw + slot * C::kRawBytes + C::kRawHalf;
-  #pragma unroll
+          // one row of scales a lane and 32 keys: a page's address, then constants of the lane
+          const uint16_t* sc = static_cast<const uint16_t*>(v ? a.c.v_scale : a.c.k_scale) +
+                               head * (v ? a.c.vs_stride[1] : a.c.ks_stride[1]);
+          const int64_t s_page = v ? a.c.vs_stride[0] : a.c.ks_stride[0], s_slot = v ? a.c.vs_stride[2] : a.c.ks_stride[2];
+          const uint32_t sb = sbase + C::kOffRaw + slot * C::kRawBytes + C::kRawHalf + lane * (HD / 16);
+#pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const int k = x * 32 + lane, key = u * 64 + k;
-            const int pg = __shfl_sync(0xffffffffu, page, k / rows);
+            const int key = u * 64 + x * 32 + lane;
+            const int pg = __shfl_sync(0xffffffffu, page, (x * 32 + lane) >> row_bits);
             const bool in_pool = key < keys && pg >= 0 && pg < a.c.pages;
-            const uint16_t* src = in_pool ? sc + pg * ss[0] + head * ss[1] + (key & (a.c.page_size - 1)) * ss[2] : sc;
-            cp_async_small<HD / 16>(sb + k * (HD / 16), src, in_pool);
+            const int at_page = in_pool ? pg : 0;
+            cp_async_small<HD / 16>(sb + x * 32 * (HD / 16), sc + at_page * s_page + (key & (a.c.page_size - 1)) * s_slot, in_pool);
           }
           asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(smem_u32(&landed[slot])) : "memory");
         }
@@ -877,42 +880,37 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
         auto convert = [&](bool v, int unit, int valid, bool edge) {
           const int slot = (v ? RH : 0) + unit % RH, rs = h % C::kRaw;
           if (!(ok = warp_wait(&landed[rs], (h / C::kRaw) & 1)) || !(ok = warp_wait(&empty[slot], ((unit / RH) & 1) ^ 1))) return;
-          const uint8_t* raw = sm + C::kOffRaw + rs * C::kRawBytes;
+          // A lane converts the same chunk of every KEYS-th key: KEYS is a multiple of 8, so the
+          // swizzle is a constant of the lane and everything moves by constants.
+          constexpr int PER = 64 * CPK / 128, KEYS = 128 / CPK;
+          const int id = hw * 32 + lane, key0 = id / CPK, ch = id % CPK;   // 16 dims: 16-bit chunks 2 ch, 2 ch + 1
+          const uint32_t raw = sbase + C::kOffRaw + rs * C::kRawBytes;
+          uint32_t src = raw + id * 16, scl = raw + C::kRawHalf + key0 * (HD / 16) + (ch >> 1) * 2;
+          const uint32_t base = sbase + slot * C::kHalf + (ch >> 2) * 8192;
+          uint32_t lo = base + sw128(key0, (2 * ch) & 7), hi = base + sw128(key0, ((2 * ch) & 7) + 1);
+#pragma unroll 2
+          for (int x = 0; x < PER; ++x) {
+            const uint4 w = ls128(src);
+            uint32_t s2 = ls16(scl);
+            s2 = key0 + x * KEYS < valid ? s2 | s2 << 16 : 0u;   // rows past the last key: +-0
+            st128(lo, dq2(w.x, 0x5140u, s2), dq2(w.x, 0x7362u, s2), dq2(w.y, 0x5140u, s2), dq2(w.y, 0x7362u, s2));
+            st128(hi, dq2(w.z, 0x5140u, s2), dq2(w.z, 0x7362u, s2), dq2(w.w, 0x5140u, s2), dq2(w.w, 0x7362u, s2));
+            src += 128 * 16;
+            scl += KEYS * (HD / 16);
+            lo += KEYS * 128;
+            hi += KEYS * 128;
+          }
           bool any_bad = false;
-          constexpr int PER = 64 * CPK / (128), BATCH = PER > 2 ? 2 : PER;
-          static_assert(PER * 128 == 64 * CPK, "the converters' shares");
-  #pragma unroll 1
-          for (int x0 = 0; x0 < PER; x0 += BATCH) {
-            uint4 x[BATCH];
-            uint32_t sc[BATCH];
-  #pragma unroll
-            for (int x1 = 0; x1 < BATCH; ++x1) {   // 16 dims: 16-bit chunks 2 ch and 2 ch + 1
-              const int idx = (x0 + x1) * 128 + hw * 32 + lane, key = idx / CPK, ch = idx % CPK;
-              x[x1] = *reinterpret_cast<const uint4*>(raw + idx * 16);
-              sc[x1] = *reinterpret_cast<const uint16_t*>(raw + C::kRawHalf + key * (HD / 16) + (ch >> 1) * 2);
-              if (key >= valid) sc[x1] = 0u;   // rows past the last key: +-0
-            }
-  #pragma unroll
-            for (int x1 = 0; x1 < BATCH; ++x1) {
-              const int idx = (x0 + x1) * 128 + hw * 32 + lane, key = idx / CPK, ch = idx % CPK;
-              const uint32_t s2 = sc[x1] | sc[x1] << 16;
-              const uint32_t in[4] = {x[x1].x, x[x1].y, x[x1].z, x[x1].w};
-              uint32_t o[8];
-  #pragma unroll
-              for (int y = 0; y < 4; ++y) {
-                o[2 * y] = dq2(in[y], 0x5140u, s2);
-                o[2 * y + 1] = dq2(in[y], 0x7362u, s2);
+          if (edge) {   // the same chunks again: what must not reach the product
+#pragma unroll 1
+            for (int x = 0; x < 2 * PER; ++x) {
+              const uint32_t at_w = (x & 1 ? hi : lo) - (x / 2 + 1) * KEYS * 128;
+              const uint4 v = ls128(at_w);
+              uint32_t o[4] = {v.x, v.y, v.z, v.w};
+              if (drop_bad<false>(o[0]) | drop_bad<false>(o[1]) | drop_bad<false>(o[2]) | drop_bad<false>(o[3])) {
+                st128(at_w, o[0], o[1], o[2], o[3]);
+                any_bad = true;
               }
-              if (edge) {
-  #pragma unroll
-                for (int y = 0; y < 8; ++y) any_bad |= drop_bad<false>(o[y]);
-              }
-              // lanes of neighbouring atoms write their two chunks in opposite order: all banks once
-              const int first = (ch >> 2) & 1;
-              uint8_t* hb = sm + slot * C::kHalf + (ch >> 2) * 8192;
-              const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
-              *reinterpret_cast<uint4*>(hb + sw128(key, ((2 * ch) & 7) + first)) = first ? hi : lo;
-              *reinterpret_cast<uint4*>(hb + sw128(key, ((2 * ch) & 7) + (first ^ 1))) = first ? lo : hi;
             }
           }
           if (any_bad) bad[unit & 7] = unit + 1;
