@@ -6,9 +6,10 @@
 // One pass over the data: a CTA holds its row in registers between the sum of squares
 // and the quantisation, so x and r are read once and h, q, s written once.  Half a warp
 // holds a chunk (8 values a thread), so the chunk's maximum is four shuffles.  Bound by HBM:
-// 2048 x 5120 fp32 in 23.2 us (5.9 TB/s, 0.90 of the measured copy rate), 8193 x 2048 fp16
+// 2048 x 5120 fp32 in 23.4 us (5.8 TB/s, 0.89 of the measured copy rate), 8193 x 2048 fp16
 // in 24.5 us (4.8 TB/s; twice the arithmetic a byte), 11 x 5120 in 2.9 us (latency).
 #include <algorithm>
+#include <type_traits>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -11,13 +11,14 @@
 //           binary search in the prefix sums, so one long prompt spreads like many short
 //           ones.  held and n_free may be updated in place: the last CTA to finish
 //           writes them, when every CTA has read them.
-//           Bound by the launch and a few dependent trips to memory: 4.4 us for 64 requests,
-//           12.4 us for 1000 requests with 118 K new tokens.
+//           Bound by the launch and a few dependent trips to memory: 4.1 us for 64 requests,
+//           11.6 us for 1000 requests with 118 K new tokens.
 // release   One CTA returns the pages of finished requests to the free stack.
 // append    Copies or quantises the rows of the new tokens into their slots.  Bound by HBM: 8191
-//           bf16 rows of 8 heads x 128 (67 MB) in 12.6 us, 5.3 TB/s (0.81 of the measured copy
+//           bf16 rows of 8 heads x 128 (67 MB) in 12.5 us, 5.4 TB/s (0.82 of the measured copy
 //           rate); 64 int8 rows in 2.1 us (latency).
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.cuh"
 

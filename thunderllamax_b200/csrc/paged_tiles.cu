@@ -33,8 +33,9 @@ namespace {
 // Measured (24 / 4 heads, dim 256): 4096 new tokens over 8192 fp16 keys 0.68 to 0.76 ms with
 // the power cap's clocks (0.81 PFLOP/s, 0.49 of the measured matrix rate); the MMAs alone
 // would take 0.43 ms in this form (16 MMAs of N = 64 and 4 of N = 256 cost 1050 to 1430
-// cycles a unit from one or two issuers); 11 rows at 100011 int8 keys 135 us (1.6 TB/s; the
-// converters are the longest loop); the mixed bf16 batch 208 us.
+// cycles a unit from one or two issuers); 11 rows at 100011 int8 keys 132 us a call (the
+// converters are the longest loop: without them 114); 2000 rows over 4000 int8 keys 344 us;
+// the mixed bf16 batch 208 us.
 //
 // Code size: the roles' loops run side by side on each scheduler, one warp each, so what
 // does not fit the instruction caches is fetched again for every unit.  Hence the loops
