@@ -41,7 +41,6 @@ class Plan:
         buf = torch.zeros(3 * self.requests + 1 + 2 * self.tokens, dtype=torch.int32, device=device)
         r, t = self.requests, self.tokens
         self.q_start, self.kv_len, self.status, self.slots, self.positions = buf.split([r + 1, r, r, t, t])
-        self._out = tuple(x.data_ptr() for x in (self.q_start, self.kv_len, self.slots, self.positions, self.status))
 
 
 class PageTable:
@@ -66,9 +65,6 @@ class PageTable:
         _i32(self.free, self.pages, "free")
         _i32(self.n_free, 1, "n_free")
         self.ws = ops.Workspace(int(_lib.lib().tlx_paged_plan_workspace_bytes()), self.table.device)
-        # (its own buffers' addresses do not change)
-        self._call, self._ws = _lib.lib().tlx_paged_plan, (self.ws.buf.data_ptr(), self.ws.nbytes)
-        self._table = (self.table.data_ptr(), self.table.stride(0), self.width)
 
     def plan(self, cached_len: torch.Tensor, new_len: torch.Tensor, plan: Plan, held_out: torch.Tensor = None,
              n_free_out: torch.Tensor = None) -> Plan:
@@ -81,10 +77,12 @@ class PageTable:
         _i32(new_len, n, "new_len")
         held_out = self.held if held_out is None else _i32(held_out, n, "held_out")
         n_free_out = self.n_free if n_free_out is None else _i32(n_free_out, 1, "n_free_out")
-        rc = self._call(
-            cached_len.data_ptr(), new_len.data_ptr(), n, self.page_size, *self._table, self.held.data_ptr(),
-            held_out.data_ptr(), self.free.data_ptr(), self.pages, self.n_free.data_ptr(), n_free_out.data_ptr(),
-            plan.tokens, *plan._out, *self._ws, ops._raw_stream(self.table))
+        rc = _lib.lib().tlx_paged_plan(
+            cached_len.data_ptr(), new_len.data_ptr(), n, self.page_size, self.table.data_ptr(), self.table.stride(0),
+            self.width, self.held.data_ptr(), held_out.data_ptr(), self.free.data_ptr(), self.pages,
+            self.n_free.data_ptr(), n_free_out.data_ptr(), plan.tokens, plan.q_start.data_ptr(),
+            plan.kv_len.data_ptr(), plan.slots.data_ptr(), plan.positions.data_ptr(), plan.status.data_ptr(),
+            self.ws.buf.data_ptr(), self.ws.nbytes, ops._raw_stream(self.table))
         check(rc, "paged_plan")
         return plan
 
@@ -103,10 +101,10 @@ class PagedCache:
     """A pool of K / V pages: k, v [pages][kv_heads][page_size][head_dim] fp16, bf16 or
     uint8 codes with fp16 scales [pages][kv_heads][page_size][head_dim / 32].  Any strides
     with contiguous rows (a [pages][page_size][kv_heads][head_dim] pool is its permuted
-    view)."""
+    view).  The object describes these very tensors: another pool is another PagedCache."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor = None, v_scale: torch.Tensor = None):
-        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or not (k.is_cuda and v.is_cuda):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or not k.is_cuda or v.device != k.device:
             raise TLXError("k and v must be CUDA [pages, kv_heads, page_size, head_dim] tensors of one dtype")
         if k.dtype not in _CACHE_DT:
             raise TLXError(f"a cache is fp16, bf16 or uint8 codes, not {k.dtype}")
@@ -116,7 +114,7 @@ class PagedCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         for s in (k_scale, v_scale):
-            if q8 and (s is None or s.dtype != torch.float16 or not s.is_cuda or s.stride(3) != 1 or
+            if q8 and (s is None or s.dtype != torch.float16 or s.device != k.device or s.stride(3) != 1 or
                        tuple(s.shape) != (*k.shape[:3], self.head_dim // 32)):
                 raise TLXError("uint8 codes need fp16 scales [pages, kv_heads, page_size, head_dim / 32]")
             if not q8 and s is not None:
@@ -164,7 +162,6 @@ class PagedAttention:
             raise TLXError(f"unsupported heads: {heads} query, {kv_heads} KV, dim {head_dim}")
         self.ws = ops.Workspace(nb, device)
         self.scale = self.head_dim ** -0.5
-        self._call, self._ws = _lib.lib().tlx_paged_attention, self.ws.buf.data_ptr()
 
     def __call__(self, cache: PagedCache, table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor,
                  q: torch.Tensor, gate: torch.Tensor = None, scale: float = None, max_new: int = None,
@@ -197,10 +194,10 @@ class PagedAttention:
             raise TLXError(f"the table has {table.shape[0]} rows for {r} requests")
         _i32(kv_len, 1, "kv_len")
         _i32(q_start, r + 1, "q_start")
-        rc = self._call(
+        rc = _lib.lib().tlx_paged_attention(
             cache._ref, table.data_ptr(), table.stride(0), table.shape[1], q_start.data_ptr(), kv_len.data_ptr(), r,
             q.data_ptr(), ops._DT[dt], qt, qh, self.heads, n, n if max_new is None else max_new,
-            self.scale if scale is None else scale, gp, gt, gh, out.data_ptr(), ot, oh, self._ws, self.ws.nbytes,
+            self.scale if scale is None else scale, gp, gt, gh, out.data_ptr(), ot, oh, self.ws.buf.data_ptr(), self.ws.nbytes,
             ops._raw_stream(q))
         check(rc, "paged_attention")
         return out
