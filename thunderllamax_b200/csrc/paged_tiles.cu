@@ -125,6 +125,13 @@ struct TilesCfg {
   static constexpr uint32_t kIdescPV = (1u << 4) | kFmt | (1u << 16) | static_cast<uint32_t>(HD >> 3) << 17 | (128u >> 4) << 24;
 };
 
+// Barriers of the P V products, by unit.  A wait names a phase by its parity alone, so it is
+// right only where the phase before (the product kPvRing units earlier) is known to be
+// complete.  The furthest look ahead is the rescale of O: at unit i a group waits for product
+// i - 1 when all it knows, from the other group's maximum of unit i - 1, is that product i - 5
+// is complete (that group saw it before it wrote P of unit i - 3).  Hence four, not two.
+constexpr int kPvRing = 4;
+
 // Positions of an item besides its units (see the schedule): with 3 / 6 / 10 the mixed batch
 // takes 309 / 250 / 246 us, with none 440.
 constexpr int kItemCost = 8;
@@ -279,8 +286,8 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
   uint64_t* s_full = empty + 6;         // [2] QK -> softmax
   uint64_t* s_free = s_full + 2;        // [2] softmax -> QK
   uint64_t* p_full = s_free + 2;        // [2] softmax -> PV
-  uint64_t* pv_done = p_full + 2;       // [2] PV -> softmax
-  uint64_t* q_full = pv_done + 2;       // softmax -> QK: Q of the next item is in
+  uint64_t* pv_done = p_full + 2;       // [kPvRing] PV -> softmax
+  uint64_t* q_full = pv_done + kPvRing; // softmax -> QK: Q of the next item is in
   uint64_t* o_free = q_full + 1;        // softmax -> PV: O of the last item is read
   uint64_t* done = o_free + 1;
   uint64_t* turn = done + 1;            // [2] QK warp -> QK warp: S of unit i is issued
@@ -297,7 +304,7 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
   First* first_at = reinterpret_cast<First*>(tmem_holder + 10);
   volatile float* m_sh = reinterpret_cast<float*>(sm + C::kOffX);   // [128]
   volatile float* l_sh = m_sh + 128;                                 // [2 items][2 groups][128]
-  static_assert((4 * 6 + 25) * 8 + 15 * 4 <= 512 && RING <= 6 && C::kRaw <= 6, "barrier area");
+  static_assert((4 * 6 + 23 + kPvRing) * 8 + 15 * 4 <= 512 && RING <= 6 && C::kRaw <= 6, "barrier area");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   griddep_launch_dependents();
@@ -354,8 +361,8 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
       mbar_init(&s_full[i], 1);
       mbar_init(&s_free[i], 4);
       mbar_init(&p_full[i], 4);
-      mbar_init(&pv_done[i], 1);
     }
+    for (int i = 0; i < kPvRing; ++i) mbar_init(&pv_done[i], 1);
     mbar_init(q_full, 4 * NG);
     mbar_init(o_free, 4 * NG);
     mbar_init(done, NG + 1);
@@ -370,6 +377,8 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
   __syncthreads();
   tc_after();
   const uint32_t tmem = *tmem_holder;
+  auto pv_bar = [&](int unit) { return &pv_done[unit % kPvRing]; };
+  auto pv_wait = [&](int unit) { return warp_wait(pv_bar(unit), (unit / kPvRing) & 1); };   // product of the unit
   auto fail = [&]() {
     atomicOr(err, ERR_MBAR_TIMEOUT);
     *abort_flag = 1u;
@@ -443,6 +452,7 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
       // (one site each for the Q load, the item's units and its end: see the note on code size)
       const bool more = i < n;
       if (more) {   // Q of the next item may follow once the last S of this one is made
+        // (S of last - 2 is complete: its group sent its maximum for this one's unit last - 1)
         if (NG == 2 && item >= 0 && (last & 1) != grp && !(ok = warp_wait(&s_full[last & 1], (last >> 1) & 1))) break;
         load_q(next);
       }
@@ -468,7 +478,8 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
           if (!(ok = warp_wait(&l_full[qd], item & 1))) break;
           l_run = l2[row] + l2[128 + row];
         }
-        if (!(ok = warp_wait(&pv_done[last & 1], (last >> 1) & 1))) break;
+        // (product last - 4 is complete: the group of unit `last` saw it at unit last - 2)
+        if (!(ok = pv_wait(last))) break;
         tc_after();
         const bool whole = at.u == 0 && last + 1 - begin_i == at.of;
         const int slot = 2 * blockIdx.x + (begin_i > 0 ? 1 : 0);   // the CTA's first part, or a later one
@@ -582,7 +593,8 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
           }
           mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
         }
-        // the row's reference maximum after the unit before this one
+        // the row's reference maximum after the unit before this one (every unit waits for the
+        // one before, so the phases come one at a time)
         float m_old = m_ref;
         if (NG == 2 && i > 0) {
           if (!(ok = warp_wait(&m_full[qd * 2 + (b ^ 1)], ((i - 1) >> 1) & 1))) break;
@@ -594,7 +606,7 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
           if (grows) m_new = mt;
           if (i > begin_i) {
             const float cor = m_old == m_new ? 1.f : ex2_approx(m_old - m_new);
-            if (!(ok = warp_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1))) break;   // O is at rest
+            if (!(ok = pv_wait(i - 1))) break;   // O is at rest (product i - 5 is complete: see kPvRing)
             tc_after();
 #pragma unroll 1
             for (int c = 0; c < HD / 16; ++c) {
@@ -620,8 +632,9 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
           m_ref = m_new;
         }
         const float off = m_ref == -INFINITY ? 0.f : -m_ref;
-        // the P buffer is free once the product that read it is done
-        if (i >= PB && !(ok = warp_wait(&pv_done[(i - PB) & 1], ((i - PB) >> 1) & 1))) break;
+        // the P buffer is free once the product that read it is done (product i - PB - 4 is
+        // complete: this group saw it at unit i - 4)
+        if (i >= PB && !(ok = pv_wait(i - PB))) break;
         if (run) {
           float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
           const float2 sc2 = make_float2(sc, sc), off2 = make_float2(off, off);
@@ -652,7 +665,7 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
         if (lane == 0) mbar_arrive(&p_full[b]);
         if (edge) {
           // bad values that were taken out of V, for the rows that see them
-          if (!(ok = warp_wait(&pv_done[b], (i >> 1) & 1))) break;
+          if (!(ok = pv_wait(i))) break;   // (product i - 4 is complete: seen at unit i - 4 + PB)
           tc_after();
           if (bad[i & 7] == i + 1)
             restore_bad_values<CT, HD>(a, at.b, at.head, k0, at.r.keys, lim_n, sm + C::kOffP + pb * C::kPBytes, row,
@@ -753,7 +766,7 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             tc_mma(tmem + C::kColO, pd + k * 2, vd + k * 128, C::kIdescPV, (!starts || k > 0) ? 1u : 0u);
-          tc_commit(&pv_done[i & 1]);
+          tc_commit(pv_bar(i));
           tc_commit(&empty[slot]);
         }
         __syncwarp();
