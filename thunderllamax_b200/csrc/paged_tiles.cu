@@ -646,9 +646,10 @@ __global__ void __launch_bounds__(TilesCfg<CT, HD>::kThreads, TilesCfg<CT, HD>::
               for (int j = 0; j < 4; ++j) {
                 // 2^(scale log2(e) s - m); a masked key's -inf gives 0
                 const float2 z = fma2(make_float2(__uint_as_float(r[8 * x + 2 * j]), __uint_as_float(r[8 * x + 2 * j + 1])), sc2, off2);
-                const float2 e = make_float2(ex2_approx(z.x), ex2_approx(z.y));
-                sums[j & 1] = add2(sums[j & 1], e);
-                w[j] = pack2<BF>(e.x, e.y);
+                w[j] = pack2<BF>(ex2_approx(z.x), ex2_approx(z.y));
+                // the sum is taken over the rounded weights: what rounding does to all of a row's
+                // weights alike cancels in the quotient
+                sums[j & 1] = add2(sums[j & 1], unpack2<BF>(w[j]));
               }
               *reinterpret_cast<uint4*>(sm + C::kOffP + pb * C::kPBytes + sw128(row, c * 4 + x)) =
                   make_uint4(w[0], w[1], w[2], w[3]);
