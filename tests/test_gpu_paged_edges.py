@@ -3,9 +3,45 @@ import pytest
 import torch
 
 from test_gpu_paged import BF16, F16, Batch, device  # noqa: F401
+from thunderllamax_b200 import paged
 
 pytestmark = pytest.mark.gpu
 CACHES = [F16, BF16, "int8"]
+
+
+# ------------------------------------------------------------- fewer rows than planned
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("new,max_new", [([3, 1], 1), ([7, 2], 3), ([60, 1], 20), ([150, 40], 40)])
+def test_rows_past_max_new_change_nothing(hd, cache, new, max_new):
+    # rows past max_new are not written, and the K and V of those tokens reach no row
+    b = Batch(new, [n + 70 for n in new], 4, 2, hd, cache, 16, seed=3, stale=False)
+    attn = paged.PagedAttention(4, 2, hd)
+
+    def run():
+        out = torch.full_like(b.q, 7.0)
+        return attn(b.store, b.table, b.q_start, b.kv_len, b.q, out=out, max_new=max_new)
+
+    clean = run()
+    for r, n in enumerate(new):
+        for i in range(min(n, max_new) + 70, n + 70):          # tokens of rows that are not asked for
+            page, off = int(b.table[r, i // 16]), i % 16
+            if cache == "int8":
+                b.store.k_scale[page, :, off] = float("nan")
+                b.store.v_scale[page, 0, off] = float("inf")
+                b.store.v_scale[page, 1, off] = float("nan")
+            else:
+                b.store.k[page, :, off] = float("nan")
+                b.store.v[page, 0, off, 3] = float("inf")
+                b.store.v[page, 1, off] = float("nan")
+    got = run()
+    assert torch.equal(got, clean)
+    at = 0
+    for n in new:
+        m = min(n, max_new)
+        assert got[at:at + m].isfinite().all() and (got[at + m:at + n] == 7).all()
+        at += n
+    assert attn.error() == 0
 
 
 # ----------------------------------------------------------------- weights that sum to one

@@ -310,9 +310,10 @@ __global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel
     // O of this warp's dims
     const uint32_t vb = kb + kOffV;
     // A key that some rows do not see must not reach them through 0 * inf or 0 * NaN: units
-    // with such keys are looked over first (of single tokens there are none).
+    // with such keys are looked over first.  (A request's only new token sees all its keys; of
+    // several planned tokens even the only row that is asked for, max_new = 1, does not.)
     bool slow = false;
-    if (at.r.n > 1 && (at.u + 1) * KT > at.r.kv - at.r.n_all + 1) {
+    if (at.r.n_all > 1 && (at.u + 1) * KT > at.r.kv - at.r.n_all + 1) {
       bool found = false;
       for (int key = max(0, at.r.kv - at.r.n_all + 1 - at.u * KT) + warp; key < KT; key += 4) {
         if constexpr (Q8) {   // (any product may overflow where the scale passes 65504 / 128)
