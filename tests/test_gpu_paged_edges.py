@@ -69,3 +69,21 @@ def test_equal_values_come_out_as_they_are(hd, cache, n, kv):
     b.q.copy_((length * hd ** -0.5).expand(n, 4, hd).to(b.dtype))
     got = b.attend()
     assert (got == 1).all(), (got - 1).abs().max()
+
+
+# ------------------------------------------------------------------------- the gate's ends
+@pytest.mark.parametrize("cache,hd", [(F16, 64), (BF16, 128), (F16, 256), (BF16, 256)])
+@pytest.mark.parametrize("n,kv", [(1, 50), (1, 9000), (40, 90), (40, 9000)])
+def test_gate_far_below_zero(cache, hd, n, kv):
+    # sigmoid(-88) is 6e-39: an infinite value stays infinite under it, a large one does not vanish
+    b = Batch([n], [kv], 4, 2, hd, cache, 16, seed=2, gate=True, stale=False)
+    b.gate.fill_(-88.0)
+    page = int(b.table[0, 0])
+    b.store.v[page, :, 0, 5] = float("inf")
+    got = b.attend()
+    assert (got[..., 5] == float("inf")).all()
+    if cache == BF16:
+        b.store.v.fill_(2.0 ** 60)
+        want = 2.0 ** 60 * torch.sigmoid(torch.tensor(-88.0, dtype=torch.float64)).item()
+        # (the fast exponential is within 2^-16 of its value at 88)
+        assert ((b.attend().double() - want).abs() <= want * (2.0 ** -8 + 2.0 ** -15)).all()

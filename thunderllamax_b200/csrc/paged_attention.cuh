@@ -209,8 +209,13 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
   if constexpr (BF) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
   else return __half22float2(bits_h2(w));
 }
-// v * sigmoid(g)
-__device__ __forceinline__ float gated(float v, float g) { return __fdividef(v, 1.f + __expf(-g)); }
+// v * sigmoid(g).  The reciprocal keeps subnormal results (the fast division is 0, or NaN for an
+// infinite v, where 1 + e^-g passes 2^126: g below -87.3).
+__device__ __forceinline__ float gated(float v, float g) {
+  float s;
+  asm("rcp.approx.f32 %0, %1;\n" : "=f"(s) : "f"(1.f + __expf(-g)));
+  return v * s;
+}
 // codes (q + 128) of bytes sel of w -> fp16x2 of fp16(q) * s, rounded once
 __device__ __forceinline__ uint32_t dq2(uint32_t w, uint32_t sel, uint32_t s2) {
   return hmul2_u(h2_bits(__hsub2(bits_h2(prmt(w, 0x64646464u, sel)), __float2half2_rn(1152.f))), s2);

@@ -471,8 +471,8 @@ __global__ void __launch_bounds__(128, RowsCfg<CT, HD>::kCtas) paged_rows_kernel
           v1 = sees ? v1 * inv : 0.f;
           if (gp) {
             const float2 x = unpack2<BF>(*reinterpret_cast<const uint32_t*>(gp + d));
-            v0 /= 1.f + __expf(-x.x);
-            v1 /= 1.f + __expf(-x.y);
+            v0 = gated(v0, x.x);
+            v1 = gated(v1, x.y);
           }
           *reinterpret_cast<uint32_t*>(dst + d) = pack2<BF>(v0, v1);
         };
