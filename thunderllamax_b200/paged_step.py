@@ -88,7 +88,9 @@ def serve(layer: PagedLayer, prompts, new_tokens: int, chunk: int, pages: int, p
         new = [min(chunk, p - d) if d < p else min(1, e - d) for d, p, e in zip(done, prompts, end)]
         n = sum(new)
         i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
-        plan = table.plan(i32(done), i32(new), paged.Plan(r, n))
+        # a finished request is planned empty: with its cached length it would take its pages again
+        cached = [d if d < e else 0 for d, e in zip(done, end)]
+        plan = table.plan(i32(cached), i32(new), paged.Plan(r, n))
         rows = lambda h: torch.randn((n, h, s.head_dim), generator=g, device="cuda").half()
         residual = torch.randn((n, s.dim), generator=g, device="cuda")
         layer(plan, table.table, rows(s.heads), rows(s.kv_heads), rows(s.kv_heads), residual, gate=rows(s.heads),
