@@ -185,6 +185,9 @@ def add_rms_norm_q8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tenso
     _check_chunk_table(sx, torch.float32, m, k, "sx")
     if rs is not None:
         _check_chunk_table(rs, torch.int32, m, k, "rs")
+    for t, name in ((out, "out"), (xq, "xq"), (sx, "sx"), (rs, "rs")):   # a host address would fault on the GPU
+        if t is not None and t.device != x.device:
+            raise TLXError(f"{name} must be on x's device")
     rc = _lib.lib().tlx_add_rms_norm_q8(x.data_ptr(), ops._DT[x.dtype], x.stride(0),
                                         None if residual is None else residual.data_ptr(), ops._DT[h_dtype],
                                         0 if residual is None else residual.stride(0), weight.data_ptr(), eps, m, k,
