@@ -26,9 +26,9 @@ NO_PAGES, TABLE_FULL, BAD_LENGTH = 1, 2, 3
 _CACHE_DT = {torch.float16: TLX_DT_F16, torch.bfloat16: TLX_DT_BF16, torch.uint8: TLX_DT_Q8}
 
 
-def _i32(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
-    if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous() or t.numel() < n:
-        raise TLXError(f"{name} must be a contiguous int32 CUDA tensor of at least {n} entries")
+def _i32(t: torch.Tensor, n: int, name: str, device: torch.device) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.device != device or not t.is_contiguous() or t.numel() < n:
+        raise TLXError(f"{name} must be a contiguous int32 tensor of at least {n} entries on {device}")
     return t
 
 
@@ -61,9 +61,10 @@ class PageTable:
         if (self.table.dtype != torch.int32 or not self.table.is_cuda or
                 tuple(self.table.shape) != (self.requests, self.width) or self.table.stride(1) != 1):
             raise TLXError("table must be a row-major int32 [requests, width] CUDA tensor")
-        _i32(self.held, self.requests, "held")
-        _i32(self.free, self.pages, "free")
-        _i32(self.n_free, 1, "n_free")
+        dev = self.table.device
+        _i32(self.held, self.requests, "held", dev)
+        _i32(self.free, self.pages, "free", dev)
+        _i32(self.n_free, 1, "n_free", dev)
         self.ws = ops.Workspace(int(_lib.lib().tlx_paged_plan_workspace_bytes()), self.table.device)
 
     def plan(self, cached_len: torch.Tensor, new_len: torch.Tensor, plan: Plan, held_out: torch.Tensor = None,
@@ -73,10 +74,14 @@ class PageTable:
         n = plan.requests
         if n > self.requests:
             raise TLXError(f"the plan has {n} requests, the table {self.requests}")
-        _i32(cached_len, n, "cached_len")
-        _i32(new_len, n, "new_len")
-        held_out = self.held if held_out is None else _i32(held_out, n, "held_out")
-        n_free_out = self.n_free if n_free_out is None else _i32(n_free_out, 1, "n_free_out")
+        dev = self.table.device
+        _i32(cached_len, n, "cached_len", dev)
+        _i32(new_len, n, "new_len", dev)
+        held_out = self.held if held_out is None else _i32(held_out, n, "held_out", dev)
+        n_free_out = self.n_free if n_free_out is None else _i32(n_free_out, 1, "n_free_out", dev)
+        for t in (plan.q_start, plan.kv_len, plan.status, plan.slots, plan.positions):
+            if t.device != dev:
+                raise TLXError("the plan must be on the table's device")
         rc = _lib.lib().tlx_paged_plan(
             cached_len.data_ptr(), new_len.data_ptr(), n, self.page_size, self.table.data_ptr(), self.table.stride(0),
             self.width, self.held.data_ptr(), held_out.data_ptr(), self.free.data_ptr(), self.pages,
@@ -91,7 +96,7 @@ class PageTable:
         n = done.numel()
         if n > self.requests:
             raise TLXError(f"done has {n} entries, the table {self.requests} requests")
-        _i32(done, 1, "done")
+        _i32(done, 1, "done", self.table.device)
         check(_lib.lib().tlx_paged_release(done.data_ptr(), n, self.table.data_ptr(), self.table.stride(0), self.width,
                                            self.held.data_ptr(), self.free.data_ptr(), self.pages,
                                            self.n_free.data_ptr(), ops._raw_stream(self.table)), "paged_release")
@@ -144,7 +149,7 @@ class PagedCache:
                 k.shape[1] != self.kv_heads or k.shape[2] != self.head_dim):
             raise TLXError("k and v must be [tokens, kv_heads, head_dim] rows of one dtype on the cache's device")
         n = k.shape[0]
-        _i32(slots, n, "slots")
+        _i32(slots, n, "slots", self.k.device)
         rc = _lib.lib().tlx_paged_append(self._ref, k.data_ptr(), v.data_ptr(), ops._DT[k.dtype], k.stride(0),
                                          k.stride(1), v.stride(0), v.stride(1), slots.data_ptr(), n, ops._raw_stream(k))
         check(rc, "paged_append")
@@ -192,8 +197,10 @@ class PagedAttention:
         r = kv_len.numel()
         if table.shape[0] < r:
             raise TLXError(f"the table has {table.shape[0]} rows for {r} requests")
-        _i32(kv_len, 1, "kv_len")
-        _i32(q_start, r + 1, "q_start")
+        _i32(kv_len, 1, "kv_len", dev)
+        _i32(q_start, r + 1, "q_start", dev)
+        if self.ws.buf.device != dev:
+            raise TLXError("the attention's workspace is on another device than the cache")
         rc = _lib.lib().tlx_paged_attention(
             cache._ref, table.data_ptr(), table.stride(0), table.shape[1], q_start.data_ptr(), kv_len.data_ptr(), r,
             q.data_ptr(), ops._DT[dt], qt, qh, self.heads, n, n if max_new is None else max_new,
