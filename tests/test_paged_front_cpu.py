@@ -168,3 +168,16 @@ def test_attention_refuses_another_device(library, workspaces, where):
         a.ws.buf.device = torch.device(where)
         a(c, **good)
     assert len(library.calls) == n
+
+
+# ------------------------------------------------------------------------ the current device
+def test_calls_need_the_current_device(monkeypatch):
+    # the default stream's handle is the same on every device: a call with another device current
+    # would launch there, on addresses of the tensors' device
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 0x100 + d, raising=False)
+    assert ops._raw_stream(tensor((1,), F32)) == 0x100
+    with pytest.raises(_lib.TLXError):
+        ops._raw_stream(tensor((1,), F32, "cuda:1"))
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 1)
+    assert ops._raw_stream(tensor((1,), F32, "cuda:1")) == 0x101

@@ -31,8 +31,13 @@ def _stream(t=None):
 
 def _raw_stream(t) -> int:
     """The current stream of t's device as an integer, without building a Stream object
-    (about 3 us a call, a third of a short kernel's whole call)."""
-    return torch._C._cuda_getCurrentRawStream(t.get_device())
+    (about 3 us a call, a third of a short kernel's whole call).  t's device has to be the
+    current one: a launch goes to the current device, and the default stream's handle does not
+    say whose it is."""
+    dev = t.get_device()
+    if dev != torch._C._cuda_getDevice():
+        raise TLXError(f"the tensors are on cuda:{dev}, which is not the current device")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def require_device():

@@ -9,9 +9,9 @@
     out = attn(cache, table.table, plan.q_start, plan.kv_len, q, gate=gate)
 
 Lengths, tables and slots stay on the device: a step reads nothing back and can be
-captured in a CUDA graph.  Tensors are only buffers, every call runs on the current
-stream of their device, and a workspace (the PageTable's, the PagedAttention's) must not
-be used by two calls that can overlap.
+captured in a CUDA graph.  Tensors are only buffers, all on one device, which has to be
+the current one; every call runs on its current stream, and a workspace (the PageTable's,
+the PagedAttention's) must not be used by two calls that can overlap.
 """
 from __future__ import annotations
 
