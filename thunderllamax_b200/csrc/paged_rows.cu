@@ -1,4 +1,5 @@
 // Rows form of the paged attention: requests with at most 16 query rows per KV head.
+#include "kernel_setup.h"
 #include "paged_attention.cuh"
 
 namespace tlx {
@@ -501,15 +502,8 @@ constexpr int kRowsCtasPerSm = 4;
 template <int CT, int HD>
 int launch_rows(AttnArgs a, void* area, int sms, cudaStream_t s, SplitSet* set) {
   using C = RowsCfg<CT, HD>;
-  static bool configured = false;
-  if (!configured) {
-    // the shared memory of all the CTAs an SM is to hold, not of one
-    if (cudaFuncSetAttribute(paged_rows_kernel<CT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess ||
-        cudaFuncSetAttribute(paged_rows_kernel<CT, HD>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) !=
-            cudaSuccess)
-      return TLX_ERR_LAUNCH;
-    configured = true;
-  }
+  static std::atomic<uint64_t> done{0};
+  if (!setup_kernel(reinterpret_cast<const void*>(paged_rows_kernel<CT, HD>), C::kSmem, done)) return TLX_ERR_LAUNCH;
   const int ctas = sms * C::kCtas;
   const int64_t items = static_cast<int64_t>(a.n_req) * a.c.kv_heads;
   a.by_item = items <= ctas;

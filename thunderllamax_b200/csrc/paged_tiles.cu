@@ -1,6 +1,7 @@
 // Tiles form of the paged attention: requests with more than 16 query rows per KV head.
 #include <cuda.h>
 
+#include "kernel_setup.h"
 #include "paged_attention.cuh"
 
 namespace tlx {
@@ -1018,15 +1019,8 @@ bool page_map(CUtensorMap* map, const tlx_paged_kv& c, const void* base, const i
 template <int CT, int HD>
 int launch_tiles(AttnArgs a, void* area, uint32_t* err, int sms, bool after_rows, cudaStream_t stream, SplitSet* set) {
   using C = TilesCfg<CT, HD>;
-  static bool configured = false;
-  if (!configured) {
-    // the shared memory of all the CTAs an SM is to hold, not of one
-    if (cudaFuncSetAttribute(paged_tiles_kernel<CT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess ||
-        cudaFuncSetAttribute(paged_tiles_kernel<CT, HD>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) !=
-            cudaSuccess)
-      return TLX_ERR_LAUNCH;
-    configured = true;
-  }
+  static std::atomic<uint64_t> done{0};
+  if (!setup_kernel(reinterpret_cast<const void*>(paged_tiles_kernel<CT, HD>), C::kSmem, done)) return TLX_ERR_LAUNCH;
   const int ctas = sms * C::kCtas;
   a.by_item = 0;
   *set = set_split(a, area, ctas, 128);
