@@ -3,6 +3,7 @@
 
 #include "kernel_setup.h"
 #include "paged_attention.cuh"
+#include "paged_schedule.h"
 
 namespace tlx {
 namespace {
@@ -137,29 +138,6 @@ constexpr int kPvRing = 4;
 // takes 309 / 250 / 246 us, with none 440.
 constexpr int kItemCost = 8;
 
-// sum over i < n of floor((a i + b) / m): the Euclid-like recursion, as a loop
-__device__ __noinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
-  int64_t s = 0;
-  while (n > 0) {
-    if (a >= m) {
-      s += (n - 1) * n / 2 * (a / m);
-      a %= m;
-    }
-    if (b >= m) {
-      s += n * (b / m);
-      b %= m;
-    }
-    const int64_t y = a * n + b;
-    if (y < m) break;
-    n = y / m;
-    b = y % m;
-    const int64_t t = m;
-    m = a;
-    a = t;
-  }
-  return s;
-}
-
 __device__ __forceinline__ int tile_tokens(const AttnArgs& a) { return 128 / a.group; }
 __device__ __forceinline__ int tile_count(const AttnArgs& a, const Req& r) {
   if (r.n < 1 || r.n * static_cast<int64_t>(a.group) <= a.rows_limit) return 0;
@@ -175,17 +153,9 @@ __device__ __forceinline__ int tile_units(const AttnArgs& a, const Req& r, int t
   return max(1, (tile_keys(a, r, tile) + 63) >> 6);
 }
 // positions of one KV head in the tiles before `tile`
-__device__ __noinline__ int64_t positions_before(const AttnArgs& a, const Req& r, int tile) {
-  const int64_t tt = tile_tokens(a), c = static_cast<int64_t>(r.kv) - r.n_all;
-  const int full = min(tile, r.n / static_cast<int>(tt));   // tiles with all their tokens
-  int64_t s = 0;
-  int i = 0;
-  if (c >= 0 && r.keys == r.kv) {   // ceil((c + (i + 1) tt) / 64), at least 1 since tt >= 1
-    s = floor_sum(full, 64, tt, c + tt + 63);
-    i = full;
-  }
-  for (; i < tile; ++i) s += tile_units(a, r, i);
-  return s + static_cast<int64_t>(tile) * kItemCost;
+__device__ __forceinline__ int64_t positions_before(const AttnArgs& a, const Req& r, int tile) {
+  return units_before(static_cast<int64_t>(r.kv) - r.n_all, tile_tokens(a), r.n, r.keys, tile) +
+         static_cast<int64_t>(tile) * kItemCost;
 }
 
 // Infinite and NaN values of V are replaced by 0 in shared memory in the units that some rows do
