@@ -1,7 +1,7 @@
 // Residual add + RMS norm + int8 tokens with one scale per 128-k chunk.
 //
 //   h = x + r,  y = h * rsqrt(mean(h^2) + eps) * w,
-//   s = max(max|y| over the chunk, 1e-6) / 127,  q = clamp(rint(y / s), +-127)
+//   s = max(max|y| over the chunk, 1e-6) * (1 / 127),  q = rint(y * (1 / s))
 //
 // One pass over the data: a CTA holds its row in registers between the sum of squares
 // and the quantisation, so x and r are read once and h, q, s written once.  Half a warp

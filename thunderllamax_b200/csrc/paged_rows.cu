@@ -18,9 +18,9 @@ namespace {
 // Bound by HBM in principle and by issue in practice for int8 caches: the kernel spends
 // about 1250 instructions a warp on a unit of 64 keys, a third of them decoding codes (60 %
 // of the issue slots, three warps a scheduler).  Measured: 64 requests of 300..16000 keys,
-// 24 / 4 heads, dim 256, int8: 148 us, 4.0 TB/s (0.61 of the measured copy rate); the same
-// lengths in bf16, 32 / 8 heads of 128: 187 us, 6.0 TB/s (0.91); one request of 4097 int8
-// keys 15.5 us with the joining kernel.  32 keys a unit for 16-bit rows of
+// 24 / 4 heads, dim 256, int8: 149 us, 4.0 TB/s (0.61 of the measured copy rate); the same
+// lengths in bf16, 32 / 8 heads of 128: 173 us, 6.5 TB/s (0.99; 177 us a call); one request of
+// 4097 int8 keys 15.8 us with the joining kernel.  32 keys a unit for 16-bit rows of
 // 256 dims and two or three stages, so that two to four CTAs share an SM.
 // Positions of an item besides its units (see the schedule): 64 requests take 179 us with
 // none, 170 with one, 171 with three.

@@ -32,12 +32,13 @@ namespace {
 // Every wait is bounded: a timeout raises the error word, all roles leave, issued MMAs
 // and copies are drained and tensor memory is freed.
 //
-// Measured (24 / 4 heads, dim 256): 4096 new tokens over 8192 fp16 keys 0.68 to 0.76 ms with
-// the power cap's clocks (0.81 PFLOP/s, 0.49 of the measured matrix rate); the MMAs alone
-// would take 0.43 ms in this form (16 MMAs of N = 64 and 4 of N = 256 cost 1050 to 1430
-// cycles a unit from one or two issuers); 11 rows at 100011 int8 keys 132 us a call (the
-// converters are the longest loop: without them 114); 2000 rows over 4000 int8 keys 344 us;
-// the mixed bf16 batch 208 us.
+// Measured (24 / 4 heads, dim 256): 4096 new tokens over 8192 fp16 keys 0.64 ms in one launch,
+// 0.77 ms in a row of calls under the power cap's clocks (0.80 PFLOP/s, 0.48 of the measured
+// matrix rate); the MMAs alone would take 0.43 ms in this form (16 MMAs of N = 64 and 4 of
+// N = 256 cost 1050 to 1430 cycles a unit from one or two issuers); 11 rows at 100011 int8 keys
+// 114 us, 130 us a call (without the converters a call takes 114 us; what makes up the rest of
+// the distance to the floor of 33 us has not been measured); 2000 rows over 4000 int8 keys
+// 330 us a call; the mixed bf16 batch 212 us, 237 us a call.
 //
 // Code size: the roles' loops run side by side on each scheduler, one warp each, so what
 // does not fit the instruction caches is fetched again for every unit.  Hence the loops
